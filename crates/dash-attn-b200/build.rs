@@ -10,6 +10,9 @@ const SOURCES: &[&str] = &[
     "generic_train.cu",
     "decode.cu",
     "rope.cu",
+    "qk_norm.cu",
+    "prefix.cu",
+    "penalize.cu",
     "sample.cu",
     "sm100.cu",
     "fwd_sm100.cu",
@@ -42,7 +45,7 @@ fn main() {
         assert!(status.success(), "nvcc failed on {}", path.display());
         objects.push(object);
     }
-    for header in ["common.cuh", "bwd_common.cuh", "sm100_ptx.cuh", "sm100_kernels.h", "sm100.h", "launch.h", "rope.h", "sample.h"] {
+    for header in ["common.cuh", "bwd_common.cuh", "sm100_ptx.cuh", "sm100_kernels.h", "sm100.h", "launch.h", "rope.h", "qk_norm.h", "prefix.h", "penalize.h", "sample.h"] {
         println!("cargo:rerun-if-changed={}", csrc.join(header).display());
     }
     let archive = out.join("libdash_attn_b200.a");

@@ -145,6 +145,75 @@ pub struct dash_sample_params {
     pub token_elem_bytes: i32,
 }
 
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct dash_rope_norm_params {
+    pub b: i32,
+    pub t: i64,
+    pub d: i32,
+    pub heads_q: i32,
+    pub heads_k: i32,
+    pub q_stride: [i64; 3],
+    pub k_stride: [i64; 3],
+    pub grad_q_stride: [i64; 3],
+    pub grad_k_stride: [i64; 3],
+    pub weight_dtype: i32,
+    pub eps: f32,
+    pub positions: *const c_void,
+    pub positions_elem_bytes: i32,
+    pub cu_seqlens: *const c_void,
+    pub cu_seqlens_len: i32,
+    pub index_elem_bytes: i32,
+    pub start: i64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct dash_attn_prefix_params {
+    pub n: i32,
+    pub p: i32,
+    pub hkv: i32,
+    pub d: i32,
+    pub v_n: i32,
+    pub v_p: i32,
+    pub v_hkv: i32,
+    pub v_d: i32,
+    pub k_stride: [i64; 4],
+    pub v_stride: [i64; 4],
+    pub lengths: *const c_void,
+    pub lengths_len: i32,
+    pub lengths_elem_bytes: i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct dash_sample_penalize_params {
+    pub dtype: i32,
+    pub b: i32,
+    pub v: i32,
+    pub row_stride: i64,
+    pub out_stride: i64,
+    pub ids: *const c_void,
+    pub ids_len: i32,
+    pub ids_elem_bytes: i32,
+    pub ids_stride: i64,
+    pub lengths: *const c_void,
+    pub prompt_lengths: *const c_void,
+    pub lengths_elem_bytes: i32,
+    pub prompt_lengths_elem_bytes: i32,
+    pub repetition: *const f32,
+    pub frequency: *const f32,
+    pub presence: *const f32,
+    pub repetition_all: f32,
+    pub frequency_all: f32,
+    pub presence_all: f32,
+    pub bias: *const c_void,
+    pub bias_dtype: i32,
+    pub bias_stride: i64,
+    pub allowed: *const c_void,
+    pub allowed_stride: i64,
+}
+
 extern "C" {
     pub fn dash_attn_forward_workspace(p: *const dash_attn_params) -> usize;
     pub fn dash_attn_backward_workspace(p: *const dash_attn_params) -> usize;
@@ -227,6 +296,68 @@ extern "C" {
         out: *mut c_void,
         workspace: *mut c_void,
         workspace_bytes: usize,
+        stream: dash_attn_stream_t,
+    ) -> c_int;
+
+    pub fn dash_rope_norm_apply(
+        rope: *const dash_rope_tables,
+        p: *const dash_rope_norm_params,
+        q: *const c_void,
+        k: *const c_void,
+        weight_q: *const c_void,
+        weight_k: *const c_void,
+        out_q: *mut c_void,
+        out_k: *mut c_void,
+        stream: dash_attn_stream_t,
+    ) -> c_int;
+
+    pub fn dash_rope_norm_backward_workspace(
+        p: *const dash_rope_norm_params,
+    ) -> usize;
+
+    pub fn dash_rope_norm_backward(
+        rope: *const dash_rope_tables,
+        p: *const dash_rope_norm_params,
+        q: *const c_void,
+        k: *const c_void,
+        weight_q: *const c_void,
+        weight_k: *const c_void,
+        grad_q: *const c_void,
+        grad_k: *const c_void,
+        dq: *mut c_void,
+        dk: *mut c_void,
+        dweight_q: *mut c_void,
+        dweight_k: *mut c_void,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        stream: dash_attn_stream_t,
+    ) -> c_int;
+
+    pub fn dash_attn_decode_shared_workspace(
+        p: *const dash_attn_decode_params,
+        x: *const dash_attn_prefix_params,
+    ) -> usize;
+
+    pub fn dash_attn_decode_shared(
+        p: *const dash_attn_decode_params,
+        x: *const dash_attn_prefix_params,
+        q: *const c_void,
+        prefix_k: *const c_void,
+        prefix_v: *const c_void,
+        k_new: *const c_void,
+        v_new: *const c_void,
+        k_cache: *mut c_void,
+        v_cache: *mut c_void,
+        out: *mut c_void,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        stream: dash_attn_stream_t,
+    ) -> c_int;
+
+    pub fn dash_sample_penalize(
+        p: *const dash_sample_penalize_params,
+        logits: *const c_void,
+        out: *mut c_void,
         stream: dash_attn_stream_t,
     ) -> c_int;
 

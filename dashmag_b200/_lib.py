@@ -115,6 +115,60 @@ class SampleParams(ctypes.Structure):
     ]
 
 
+class QkNormParams(ctypes.Structure):
+    """``dash_rope_norm_params``."""
+    _fields_ = [
+        ("b", i32),
+        ("t", i64),
+        ("d", i32),
+        ("heads_q", i32), ("heads_k", i32),
+        ("q_stride", i64 * 3), ("k_stride", i64 * 3),
+        ("grad_q_stride", i64 * 3), ("grad_k_stride", i64 * 3),
+        ("weight_dtype", i32),
+        ("eps", f32),
+        ("positions", vp),
+        ("positions_elem_bytes", i32),
+        ("cu_seqlens", vp),
+        ("cu_seqlens_len", i32),
+        ("index_elem_bytes", i32),
+        ("start", i64),
+    ]
+
+
+class PrefixParams(ctypes.Structure):
+    """``dash_attn_prefix_params``."""
+    _fields_ = [
+        ("n", i32), ("p", i32),
+        ("hkv", i32), ("d", i32), ("v_n", i32), ("v_p", i32), ("v_hkv", i32), ("v_d", i32),
+        ("k_stride", i64 * 4), ("v_stride", i64 * 4),
+        ("lengths", vp),
+        ("lengths_len", i32),
+        ("lengths_elem_bytes", i32),
+    ]
+
+
+class PenalizeParams(ctypes.Structure):
+    """``dash_sample_penalize_params``."""
+    _fields_ = [
+        ("dtype", i32),
+        ("b", i32), ("v", i32),
+        ("row_stride", i64), ("out_stride", i64),
+        ("ids", vp),
+        ("ids_len", i32), ("ids_elem_bytes", i32),
+        ("ids_stride", i64),
+        ("lengths", vp),
+        ("prompt_lengths", vp),
+        ("lengths_elem_bytes", i32), ("prompt_lengths_elem_bytes", i32),
+        ("repetition", vp), ("frequency", vp), ("presence", vp),
+        ("repetition_all", f32), ("frequency_all", f32), ("presence_all", f32),
+        ("bias", vp),
+        ("bias_dtype", i32),
+        ("bias_stride", i64),
+        ("allowed", vp),
+        ("allowed_stride", i64),
+    ]
+
+
 # The two parameter structs' fields in order, as native struct formats: one pack call fills a struct in a microsecond and a
 # half where a field at a time (five of them arrays) takes six or seven, a fifth of a short call's host time.
 PARAMS_FORMAT = struct.Struct("@12i 20q iPi2i2qPP5i2qifi")
@@ -149,6 +203,12 @@ PROTOTYPES = {
     "dash_attn_decode_append_rope_workspace": (ctypes.c_size_t, [ctypes.POINTER(DecodeParams)]),
     "dash_attn_decode_append_rope": (ctypes.c_int, [ctypes.POINTER(DecodeParams), ctypes.POINTER(RopeTables), vp, i32,
                                                     vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp]),
+    "dash_rope_norm_apply": (ctypes.c_int, [ctypes.POINTER(RopeTables), ctypes.POINTER(QkNormParams), vp, vp, vp, vp, vp, vp, vp]),
+    "dash_rope_norm_backward_workspace": (ctypes.c_size_t, [ctypes.POINTER(QkNormParams)]),
+    "dash_rope_norm_backward": (ctypes.c_int, [ctypes.POINTER(RopeTables), ctypes.POINTER(QkNormParams), *[vp] * 11, ctypes.c_size_t, vp]),
+    "dash_attn_decode_shared_workspace": (ctypes.c_size_t, [ctypes.POINTER(DecodeParams), ctypes.POINTER(PrefixParams)]),
+    "dash_attn_decode_shared": (ctypes.c_int, [ctypes.POINTER(DecodeParams), ctypes.POINTER(PrefixParams), *[vp] * 9, ctypes.c_size_t, vp]),
+    "dash_sample_penalize": (ctypes.c_int, [ctypes.POINTER(PenalizeParams), vp, vp, vp]),
     "dash_sample_workspace": (ctypes.c_size_t, [ctypes.POINTER(SampleParams)]),
     "dash_sample": (ctypes.c_int, [ctypes.POINTER(SampleParams), vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp]),
     "dash_attn_decode_static": (ctypes.c_int, [ctypes.POINTER(DecodeParams), vp, vp, vp, vp, vp]),

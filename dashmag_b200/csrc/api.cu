@@ -13,6 +13,9 @@
 #include "../../include/dash_attn.h"
 #include "common.cuh"
 #include "launch.h"
+#include "penalize.h"
+#include "prefix.h"
+#include "qk_norm.h"
 #include "rope.h"
 #include "sample.h"
 #include "sm100.h"
@@ -598,6 +601,278 @@ int dash_attn_decode_append_rope(const dash_attn_decode_params *p, const dash_ro
     dash_attn_decode_params rotated = *p;
     rotated.q_stride[0] = (int64_t)p->hq * p->d; rotated.q_stride[1] = p->d; rotated.q_stride[2] = 1;
     return decode_impl(op, &rotated, q_rot, k_rot, v_new, k_cache, v_cache, out, workspace, workspace_bytes, stream_);
+}
+
+// ------------------------------------------------------------------------------------------------
+// The norm of queries and keys with the rotation
+// ------------------------------------------------------------------------------------------------
+static int check_qk_norm(const char *op, const dash_rope_tables *r, const dash_rope_norm_params *p) {
+    if (!p) return fail(DASH_ATTN_INVALID, "%s: null parameters", op);
+    if (p->b < 0 || p->t < 0 || p->d < 0 || p->heads_q < 0 || p->heads_k < 0) return fail(DASH_ATTN_INVALID, "%s: no dimension may be negative", op);
+    int rc = check_rope(op, r, p->d);
+    if (rc != DASH_ATTN_OK) return rc;
+    if (p->d > 256) return fail(DASH_ATTN_UNSUPPORTED, "%s: head dimension %d: this library takes up to 256", op, p->d);
+    if (p->weight_dtype != r->dtype && p->weight_dtype != DASH_ATTN_F32)
+        return fail(DASH_ATTN_INVALID, "%s: weights of dtype code %d beside tensors of code %d; theirs or f32", op, p->weight_dtype, r->dtype);
+    if (!(p->eps >= 0.f && std::isfinite(p->eps))) return fail(DASH_ATTN_INVALID, "%s: eps must be finite and >= 0, got %g", op, (double)p->eps);
+    if (p->positions && p->positions_elem_bytes != 4 && p->positions_elem_bytes != 8)
+        return fail(DASH_ATTN_INVALID, "Rope: positions of %d bytes; i32 or i64", p->positions_elem_bytes);
+    if (!p->positions && p->cu_seqlens) {
+        if (p->index_elem_bytes != 4 && p->index_elem_bytes != 8) return fail(DASH_ATTN_INVALID, "Rope: offsets of %d bytes; i32 or i64", p->index_elem_bytes);
+        if (p->cu_seqlens_len < 1) return fail(DASH_ATTN_INVALID, "Rope: the offsets hold at least the first 0");
+        if (p->b != 1) return fail(DASH_ATTN_INVALID, "%s: packed sequences lie along the time, B = 1", op);
+    }
+    const int64_t heads = (int64_t)p->heads_q + p->heads_k;
+    if (p->t > (int64_t(1) << 40)) return fail(DASH_ATTN_UNSUPPORTED, "%s: %lld tokens", op, (long long)p->t);
+    if (p->b * p->t * heads * p->d != 0 && !p->positions && !p->cu_seqlens && (p->start < 0 || p->start > r->len - p->t))
+        return fail(DASH_ATTN_INVALID, "Rope: positions %lld..%lld of %lld", (long long)p->start, (long long)(p->start + p->t), (long long)r->len);
+    return DASH_ATTN_OK;
+}
+
+static dash::NormArgs norm_args(const dash_rope_tables *r, const dash_rope_norm_params *p) {
+    dash::NormArgs a{};
+    a.b = p->b; a.t = p->t; a.d = p->d; a.dim = r->dim; a.eps = p->eps;
+    a.w_f32 = p->weight_dtype == DASH_ATTN_F32;
+    a.cos = r->cos; a.sin = r->sin; a.len = r->len;
+    a.positions = p->positions; a.pos_bytes = p->positions_elem_bytes;
+    if (!p->positions && p->cu_seqlens) {
+        a.cu = p->cu_seqlens; a.cu_bytes = p->index_elem_bytes; a.sequences = p->cu_seqlens_len - 1;
+    }
+    a.start = p->start;
+    auto strides = [](dash::NormTensor &t, int heads, const int64_t *x, const int64_t *g) {
+        t.heads = heads;
+        t.sb = x[0]; t.st = x[1]; t.sh = x[2];
+        t.gb = g[0]; t.gt = g[1]; t.gh = g[2];
+    };
+    strides(a.q, p->heads_q, p->q_stride, p->grad_q_stride);
+    strides(a.k, p->heads_k, p->k_stride, p->grad_k_stride);
+    return a;
+}
+
+int dash_rope_norm_apply(const dash_rope_tables *r, const dash_rope_norm_params *p, const void *q, const void *k, const void *weight_q,
+                       const void *weight_k, void *out_q, void *out_k, dash_attn_stream_t stream_) {
+    const char *op = "qk_norm";
+    g_error.clear();
+    int rc = check_qk_norm(op, r, p);
+    if (rc != DASH_ATTN_OK) return rc;
+    if (p->b * p->t * ((int64_t)p->heads_q + p->heads_k) == 0) return DASH_ATTN_OK;
+    if ((p->heads_q && (!q || !out_q)) || (p->heads_k && (!k || !out_k))) return fail(DASH_ATTN_INVALID, "%s: a tensor pointer is null", op);
+    dash::NormArgs a = norm_args(r, p);
+    a.q.x = q; a.q.w = weight_q; a.q.out = out_q;
+    a.k.x = k; a.k.w = weight_k; a.k.out = out_k;
+    int launches = 0;
+    cudaError_t e = dash::launch_qk_norm(r->dtype, a, reinterpret_cast<cudaStream_t>(stream_), &launches);
+    g_probe[DASH_ATTN_PROBE_KERNEL_LAUNCHES] += launches;
+    if (e != cudaSuccess) return cuda_fail(op, e);
+    return DASH_ATTN_OK;
+}
+
+size_t dash_rope_norm_backward_workspace(const dash_rope_norm_params *p) {
+    if (!p || p->b <= 0 || p->t <= 0 || p->d <= 0 || p->heads_q < 0 || p->heads_k < 0 || p->heads_q + (int64_t)p->heads_k == 0) return 0;
+    return align256(sizeof(float) * dash::qk_norm_part_floats(p->d));
+}
+
+int dash_rope_norm_backward(const dash_rope_tables *r, const dash_rope_norm_params *p, const void *q, const void *k, const void *weight_q,
+                          const void *weight_k, const void *grad_q, const void *grad_k, void *dq, void *dk, void *dweight_q,
+                          void *dweight_k, void *workspace, size_t workspace_bytes, dash_attn_stream_t stream_) {
+    const char *op = "qk_norm_backward";
+    g_error.clear();
+    int rc = check_qk_norm(op, r, p);
+    if (rc != DASH_ATTN_OK) return rc;
+    cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+    if (p->b * p->t * ((int64_t)p->heads_q + p->heads_k) == 0) {   // no token: the weights' gradients are empty sums
+        const size_t bytes = (size_t)p->d * elem_bytes(p->weight_dtype);
+        cudaError_t e = cudaSuccess;
+        if (dweight_q) e = cudaMemsetAsync(dweight_q, 0, bytes, stream);
+        if (e == cudaSuccess && dweight_k) e = cudaMemsetAsync(dweight_k, 0, bytes, stream);
+        return e == cudaSuccess ? DASH_ATTN_OK : cuda_fail(op, e);
+    }
+    if ((p->heads_q && (!q || !grad_q || !dq)) || (p->heads_k && (!k || !grad_k || !dk))) return fail(DASH_ATTN_INVALID, "%s: a tensor pointer is null", op);
+    if ((rc = check_workspace(op, workspace, workspace_bytes, dash_rope_norm_backward_workspace(p))) != DASH_ATTN_OK) return rc;
+    dash::NormArgs a = norm_args(r, p);
+    a.q.x = q; a.q.g = grad_q; a.q.w = weight_q; a.q.out = dq; a.q.dw = dweight_q;
+    a.k.x = k; a.k.g = grad_k; a.k.w = weight_k; a.k.out = dk; a.k.dw = dweight_k;
+    a.part = static_cast<float *>(workspace);
+    int launches = 0;
+    cudaError_t e = dash::launch_qk_norm_backward(r->dtype, a, stream, &launches);
+    g_probe[DASH_ATTN_PROBE_KERNEL_LAUNCHES] += launches;
+    if (e != cudaSuccess) return cuda_fail(op, e);
+    return DASH_ATTN_OK;
+}
+
+// ------------------------------------------------------------------------------------------------
+// The decoding step over shared prompts
+// ------------------------------------------------------------------------------------------------
+static int check_prefix(const char *op, const dash_attn_decode_params *p, const dash_attn_prefix_params *x) {
+    int rc = check_decode(p, op);
+    if (rc != DASH_ATTN_OK) return rc;
+    if (!x) return fail(DASH_ATTN_INVALID, "%s: null prompt parameters", op);
+    if (x->n < 0 || x->p < 0) return fail(DASH_ATTN_INVALID, "%s: the prompts are [N, P, Hkv, D], no dimension negative", op);
+    if (x->v_n != x->n || x->v_p != x->p || x->v_hkv != x->hkv || x->v_d != x->d)
+        return fail(DASH_ATTN_INVALID, "%s: the prompts' key and value must have one shape", op);
+    if (x->hkv != p->hkv || x->d != p->d)
+        return fail(DASH_ATTN_INVALID, "%s: the prompts' [Hkv, D] = [%d, %d] must be the cache's [%d, %d]", op, x->hkv, x->d, p->hkv, p->d);
+    if (p->b > 0 && (x->n == 0 || p->b % x->n != 0))
+        return fail(DASH_ATTN_INVALID, "%s: the batch (%d) must be a multiple of the prompts (%d)", op, p->b, x->n);
+    if (x->lengths) {
+        if (x->lengths_len != x->n) return fail(DASH_ATTN_INVALID, "%s: the prompts' lengths are [N] = [%d]", op, x->n);
+        if (x->lengths_elem_bytes != 4 && x->lengths_elem_bytes != 8)
+            return fail(DASH_ATTN_INVALID, "%s: the prompts' lengths are 4- or 8-byte integers", op);
+    }
+    if ((int64_t)x->p + p->s + 1 > 0x3fffffff)
+        return fail(DASH_ATTN_UNSUPPORTED, "%s: P + S = %lld: this library takes up to 2^30", op, (long long)x->p + p->s);
+    return DASH_ATTN_OK;
+}
+
+// The parts of a call in the workspace: the prompts' (of as many runs as whichever kernels take it cut), then the own chunks'.
+struct PrefixSpace {
+    int tensor, generic, chunk, chunks;
+    size_t part_o, part_lse, own_o, own_lse;   // bytes
+};
+static PrefixSpace prefix_space(const dash_attn_decode_params *p, const dash_attn_prefix_params *x) {
+    PrefixSpace s{};
+    const int each = p->b / x->n;
+    s.tensor = dash::sm100_prefix_splits(p->dtype, scale_for(p->has_scale, p->scale, p->d), x->n, each, x->p, p->hq, p->hkv, p->d);
+    s.generic = dash::prefix_generic_splits(x->n, each, x->p, p->hq, p->hkv);
+    const size_t rows = (size_t)p->b * p->hq, splits = (size_t)std::max(s.tensor, s.generic);
+    s.part_o = align256(sizeof(float) * rows * splits * p->d);
+    s.part_lse = align256(sizeof(float) * rows * splits);
+    if (p->s > 0) {
+        decode_plan(p, &s.chunk, &s.chunks);
+        s.own_o = align256(sizeof(float) * rows * s.chunks * p->d);
+        s.own_lse = align256(sizeof(float) * rows * s.chunks);
+    }
+    return s;
+}
+
+size_t dash_attn_decode_shared_workspace(const dash_attn_decode_params *p, const dash_attn_prefix_params *x) {
+    if (!p || !x || check_prefix("attention_decode_shared", p, x) != DASH_ATTN_OK || (int64_t)p->b * p->hq * p->d == 0) return 0;
+    if (x->p == 0) return dash_attn_decode_workspace(p);
+    const PrefixSpace s = prefix_space(p, x);
+    return s.part_o + s.part_lse + s.own_o + s.own_lse;
+}
+
+int dash_attn_decode_shared(const dash_attn_decode_params *p, const dash_attn_prefix_params *x, const void *q, const void *prefix_k,
+                            const void *prefix_v, const void *k_new, const void *v_new, void *k_cache, void *v_cache, void *out,
+                            void *workspace, size_t workspace_bytes, dash_attn_stream_t stream_) {
+    const bool append = k_new || v_new;
+    const char *op = append ? "attention_decode_shared_append" : "attention_decode_shared";
+    g_error.clear();
+    int rc = check_prefix(op, p, x);
+    if (rc != DASH_ATTN_OK) return rc;
+    if (append && !p->lengths) return fail(DASH_ATTN_INVALID, "%s: the lengths are needed: they say where each sequence's new row goes", op);
+    if (append && (!k_new || !v_new)) return fail(DASH_ATTN_INVALID, "%s: a new row is null", op);
+    if ((int64_t)p->b * p->hq * p->d == 0) return DASH_ATTN_OK;
+    if (x->p == 0) return decode_impl(op, p, q, k_new, v_new, k_cache, v_cache, out, workspace, workspace_bytes, stream_);
+    if (!out) return fail(DASH_ATTN_INVALID, "%s: the output is null", op);
+    if (!q || !prefix_k || !prefix_v || (p->s > 0 && (!k_cache || !v_cache))) return fail(DASH_ATTN_INVALID, "%s: a tensor pointer is null", op);
+    if ((rc = check_workspace(op, workspace, workspace_bytes, dash_attn_decode_shared_workspace(p, x))) != DASH_ATTN_OK) return rc;
+    cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+    const PrefixSpace s = prefix_space(p, x);
+    char *at = static_cast<char *>(workspace);
+
+    dash::PrefixArgs a{};
+    a.n = x->n; a.each = p->b / x->n; a.p = x->p; a.hq = p->hq; a.hkv = p->hkv; a.d = p->d;
+    a.scale = scale_for(p->has_scale, p->scale, p->d);
+    a.q = q;
+    a.q_sb = p->q_stride[0]; a.q_sh = p->q_stride[1]; a.q_sd = p->q_stride[2];
+    a.k = view(prefix_k, x->k_stride);
+    a.v = view(prefix_v, x->v_stride);
+    a.part_o = reinterpret_cast<float *>(at);
+    a.part_lse = reinterpret_cast<float *>(at + s.part_o);
+    const int64_t none = (int64_t)x->p + p->s + 1;
+    const int64_t left = p->has_window && p->window_left >= 0 && p->window_left < none ? p->window_left : none;
+    a.reach = dash::PrefixReach{x->lengths, p->lengths, x->lengths_elem_bytes, p->lengths_elem_bytes, x->p, p->s, append ? 1 : 0, (int)left};
+
+    dash::DecodeArgs own{};
+    own.b = p->b; own.s = p->s; own.hq = p->hq; own.hkv = p->hkv; own.d = p->d;
+    own.scale = a.scale;
+    own.q = q;
+    own.q_sb = a.q_sb; own.q_sh = a.q_sh; own.q_sd = a.q_sd;
+    own.k = view(k_cache, p->k_stride);
+    own.v = view(v_cache, p->v_stride);
+    own.lengths = p->lengths;
+    own.len_bytes = p->lengths_elem_bytes;
+    own.left = (int)std::min<int64_t>(left, (int64_t)p->s + 1);
+    own.chunk = s.chunk; own.splits = s.chunks;
+    own.part_o = reinterpret_cast<float *>(at + s.part_o + s.part_lse);
+    own.part_lse = reinterpret_cast<float *>(at + s.part_o + s.part_lse + s.own_o);
+    own.out = out;
+    own.k_new = k_new;
+    own.v_new = v_new;
+
+    int launches = 0;
+    cudaError_t e = cudaSuccess;
+    const bool both = p->s > 0;
+    if (both) e = dash::launch_decode_parts(p->dtype, own, decode_vectors(p, q, k_new, v_new, k_cache, v_cache), stream, &launches);
+    if (e == cudaSuccess) {
+        if (s.tensor > 0 && !g_force_generic.load() && dash::sm100_prefix_takes(a)) {
+            a.splits = s.tensor;
+            if (!dash::sm100_prefix(p->dtype, a, both, stream, &launches, &e)) {
+                g_probe[DASH_ATTN_PROBE_KERNEL_LAUNCHES] += launches;
+                return fail(DASH_ATTN_CUDA, "%s: the driver refused a TMA tensor map over the inputs", op);
+            }
+            g_probe[DASH_ATTN_PROBE_TENSOR_CORE_RUNS] += 1;
+        } else {
+            a.splits = s.generic;
+            e = dash::launch_prefix_generic(p->dtype, a, both, stream, &launches);
+            g_probe[DASH_ATTN_PROBE_GENERIC_RUNS] += 1;
+        }
+    }
+    if (e == cudaSuccess) {
+        const dash::PrefixMergeArgs m{(int64_t)p->b * p->hq, p->hq, p->d, a.splits, a.part_o, a.part_lse, own, out};
+        e = dash::launch_prefix_merge(p->dtype, m, stream, &launches);
+    }
+    g_probe[DASH_ATTN_PROBE_KERNEL_LAUNCHES] += launches;
+    if (e != cudaSuccess) return cuda_fail(op, e);
+    return DASH_ATTN_OK;
+}
+
+// ------------------------------------------------------------------------------------------------
+// The rules on a step's logits
+// ------------------------------------------------------------------------------------------------
+int dash_sample_penalize(const dash_sample_penalize_params *p, const void *logits, void *out, dash_attn_stream_t stream_) {
+    const char *op = "penalize";
+    g_error.clear();
+    if (!p) return fail(DASH_ATTN_INVALID, "%s: null parameters", op);
+    if (p->dtype != DASH_ATTN_F32 && p->dtype != DASH_ATTN_BF16 && p->dtype != DASH_ATTN_F16)
+        return fail(DASH_ATTN_INVALID, "%s: logits must be f32, bf16 or f16, got code %d", op, p->dtype);
+    if (p->b < 0 || p->v < 0 || p->ids_len < 0) return fail(DASH_ATTN_INVALID, "%s: logits must be [B, V] and the ids [B, T], no dimension negative", op);
+    if (p->v > (1 << 30)) return fail(DASH_ATTN_UNSUPPORTED, "%s: a vocabulary of %d tokens; up to 2^30 are taken", op, p->v);
+    if (p->ids) {
+        if (p->ids_elem_bytes != 4 && p->ids_elem_bytes != 8) return fail(DASH_ATTN_INVALID, "%s: ids of %d bytes; i32 or i64", op, p->ids_elem_bytes);
+        if (p->lengths && p->lengths_elem_bytes != 4 && p->lengths_elem_bytes != 8)
+            return fail(DASH_ATTN_INVALID, "%s: lengths of %d bytes; i32 or i64", op, p->lengths_elem_bytes);
+        if (p->prompt_lengths && p->prompt_lengths_elem_bytes != 4 && p->prompt_lengths_elem_bytes != 8)
+            return fail(DASH_ATTN_INVALID, "%s: prompt lengths of %d bytes; i32 or i64", op, p->prompt_lengths_elem_bytes);
+    }
+    if (!p->repetition && !(p->repetition_all > 0.f && std::isfinite(p->repetition_all)))
+        return fail(DASH_ATTN_INVALID, "%s: the repetition penalty must be finite and > 0, got %g", op, (double)p->repetition_all);
+    if ((!p->frequency && !std::isfinite(p->frequency_all)) || (!p->presence && !std::isfinite(p->presence_all)))
+        return fail(DASH_ATTN_INVALID, "%s: the frequency and presence penalties must be finite, got %g and %g", op, (double)p->frequency_all,
+                    (double)p->presence_all);
+    if (p->bias && p->bias_dtype != p->dtype && p->bias_dtype != DASH_ATTN_F32)
+        return fail(DASH_ATTN_INVALID, "%s: a bias of dtype code %d beside logits of code %d; theirs or f32", op, p->bias_dtype, p->dtype);
+    if (p->b == 0 || p->v == 0) return DASH_ATTN_OK;
+    if (!logits || !out) return fail(DASH_ATTN_INVALID, "%s: a tensor pointer is null", op);
+    if (p->b > 1 && p->out_stride < p->v) return fail(DASH_ATTN_INVALID, "%s: out's rows overlap", op);
+    dash::PenalizeArgs a{};
+    a.logits = logits; a.out = out; a.b = p->b; a.v = p->v;
+    a.stride = p->row_stride; a.out_stride = p->out_stride;
+    if (p->ids && p->ids_len > 0) {
+        a.ids = p->ids; a.t = p->ids_len; a.ids_bytes = p->ids_elem_bytes; a.ids_stride = p->ids_stride;
+        a.lengths = p->lengths; a.prompt = p->prompt_lengths;
+        a.lengths_bytes = p->lengths_elem_bytes; a.prompt_bytes = p->prompt_lengths_elem_bytes;
+    }
+    a.repetition = p->repetition; a.frequency = p->frequency; a.presence = p->presence;
+    a.repetition_all = p->repetition_all; a.frequency_all = p->frequency_all; a.presence_all = p->presence_all;
+    a.bias = p->bias; a.bias_f32 = p->bias_dtype == DASH_ATTN_F32; a.bias_stride = p->bias_stride;
+    a.allowed = static_cast<const uint32_t *>(p->allowed); a.allowed_stride = p->allowed_stride;
+    int launches = 0;
+    cudaError_t e = dash::launch_penalize(p->dtype, a, reinterpret_cast<cudaStream_t>(stream_), &launches);
+    g_probe[DASH_ATTN_PROBE_KERNEL_LAUNCHES] += launches;
+    if (e != cudaSuccess) return cuda_fail(op, e);
+    return DASH_ATTN_OK;
 }
 
 // ------------------------------------------------------------------------------------------------

@@ -269,6 +269,25 @@ __device__ __forceinline__ int warp_max_i(int x) {
     return x;
 }
 
+// Which keys of a shared prompt a sequence of the batch sees, when its own keys (a decoding step's cache) follow the prompt's: the
+// query is the last of its own keys and sees from `left` positions before that one on, so of the prompt [lo, its length).
+struct PrefixReach {
+    const void *prompt;    // [N] the prompts' lengths, or null: `p` each
+    const void *lengths;   // [B] what each sequence holds of its own, or null: `s` each
+    int prompt_bytes, lengths_bytes;
+    int p, s;              // the most that a prompt, that a sequence holds
+    int append;            // 1: the step's own row comes on top of `lengths`
+    int left;              // clamped to p + s + 1 = no bound
+};
+__device__ __forceinline__ void prefix_bounds(const PrefixReach &r, int prompt, int64_t sequence, int &lo, int &hi) {
+    hi = r.p;
+    if (r.prompt) hi = min(max(load_index(r.prompt, r.prompt_bytes, prompt), 0), r.p);
+    int own = r.s;
+    if (r.lengths) own = (int)min((int64_t)max(load_index(r.lengths, r.lengths_bytes, (int)sequence), 0) + r.append, (int64_t)r.s);
+    lo = max(0, hi + own - 1 - r.left);
+    if (lo >= hi) { lo = r.p; hi = 0; }
+}
+
 // ---------------------------------------------------------------------------------------------
 // Kernels of one call that run side by side
 // ---------------------------------------------------------------------------------------------

@@ -1189,13 +1189,14 @@ static int decode_cluster(const DecodeArgs &a, bool narrow) {
     }
     return best;
 }
+// (`merged` null: chunks, whose parts somebody else merges.)
 template <typename T, int DFULL>
 static cudaError_t split_mma(const DecodeArgs &a, cudaStream_t stream, bool *merged) {
     const int group = a.hq / a.hkv;
     const bool wide = group > 8;
     // (A cluster stores its outputs eight bytes at a time, the merge one element: it takes any address.)
     const bool whole = reinterpret_cast<uintptr_t>(a.out) % 8 == 0;
-    if (const int cluster = wide || !whole ? 0 : decode_cluster(a, MmaType<T>::NARROW)) {
+    if (const int cluster = wide || !whole || !merged ? 0 : decode_cluster(a, MmaType<T>::NARROW)) {
         const long long warps = (long long)a.hkv * cluster * CLUSTER_WARPS;
         const cudaError_t e = split_mma_w<T, DFULL, false, CLUSTER_WARPS, true>(a, warps, cluster, stream);
         *merged = e == cudaSuccess;
@@ -1228,14 +1229,14 @@ bool decode_fuses_rope(int dtype, const DecodeArgs &a, bool vector_ok) {
     return dtype != 0 && decode_uses_mma(2, a, vector_ok) && a.rope_dim % 16 == 0 && aligned(a.rope_cos) && aligned(a.rope_sin);
 }
 
+// The split pass; *merged: it left the outputs, and no parts.
 template <typename T>
-static cudaError_t decode_t(const DecodeArgs &a, bool vector_ok, cudaStream_t stream, int *launches) {
+static cudaError_t split_t(const DecodeArgs &a, bool vector_ok, cudaStream_t stream, bool *merged) {
     cudaError_t e;
     const bool mma = decode_uses_mma(sizeof(T), a, vector_ok);
-    bool merged = false;
-    if (mma && a.d == 128) e = split_mma<T, 128>(a, stream, &merged);
-    else if (mma && a.d == 64) e = split_mma<T, 64>(a, stream, &merged);
-    else if (mma && a.d == 256) e = split_mma<T, 256>(a, stream, &merged);
+    if (mma && a.d == 128) e = split_mma<T, 128>(a, stream, merged);
+    else if (mma && a.d == 64) e = split_mma<T, 64>(a, stream, merged);
+    else if (mma && a.d == 256) e = split_mma<T, 256>(a, stream, merged);
     else if (vector_ok && a.d == 64) e = split_vec<T, 64>(a, stream);
     else if (vector_ok && a.d == 128) e = split_vec<T, 128>(a, stream);
     else if (vector_ok && a.d == 256) e = split_vec<T, 256>(a, stream);
@@ -1245,6 +1246,13 @@ static cudaError_t decode_t(const DecodeArgs &a, bool vector_ok, cudaStream_t st
         decode_split_scalar_kernel<T><<<grid, DEC_WARPS * 32, 0, stream>>>(a);
         e = cudaGetLastError();
     }
+    return e;
+}
+
+template <typename T>
+static cudaError_t decode_t(const DecodeArgs &a, bool vector_ok, cudaStream_t stream, int *launches) {
+    bool merged = false;
+    const cudaError_t e = split_t<T>(a, vector_ok, stream, &merged);
     *launches += 1;
     if (e != cudaSuccess || merged) return e;
     *launches += 1;
@@ -1271,6 +1279,15 @@ cudaError_t launch_decode(int dtype, const DecodeArgs &a, bool vector_ok, cudaSt
         case 0: return decode_t<float>(a, vector_ok, stream, launches);
         case 1: return decode_t<__nv_bfloat16>(a, vector_ok, stream, launches);
         default: return decode_t<__half>(a, vector_ok, stream, launches);
+    }
+}
+
+cudaError_t launch_decode_parts(int dtype, const DecodeArgs &a, bool vector_ok, cudaStream_t stream, int *launches) {
+    *launches += 1;
+    switch (dtype) {
+        case 0: return split_t<float>(a, vector_ok, stream, nullptr);
+        case 1: return split_t<__nv_bfloat16>(a, vector_ok, stream, nullptr);
+        default: return split_t<__half>(a, vector_ok, stream, nullptr);
     }
 }
 

@@ -80,6 +80,7 @@ struct Barriers {
     uint64_t s_full[NT][2], p_full[NT][2];   // per S buffer
     uint64_t o_tail[NT], o_done[NT];   // the last P V but one of the tile has completed / the last one has
     uint64_t turn[4][NT];              // per scheduler: which tile's softmax warp may run its exponentials
+    uint64_t v_tail;                   // PREFIX: the rows of the last V tile that are past the prompt's end are zero
 };
 
 struct Shared {
@@ -128,11 +129,16 @@ __device__ __noinline__ void rescale_accumulator(uint32_t taddr, float factor) {
 
 // SPLIT: the block sweeps one of a.splits runs of its tiles' keys and leaves parts for the merge.  (An instance of its own: short
 // sweeps that are not split paid for its code, 20 packed sequences of 3000 tokens, 16 / 16 heads of 128, 30.3 us against 29.0.)
-template <typename T, int HD, bool SPLIT>
+// PREFIX: split, over a decoding step's shared prompts (prefix.cu): batch element = prompt, token = sequence of it, intervals
+// from a.reach.  What lies past a prompt's end may be anything: its scores are masked as any others, and its values, which P's zeros would
+// not keep out if they are not finite, are cleared in shared memory before they are multiplied.
+enum FwdForm { WHOLE, SPLITS, PREFIXES };
+template <typename T, int HD, FwdForm FORM>
 __global__ void __launch_bounds__(THREADS, 1)
 fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o, const Sm100FwdArgs a) {
     extern __shared__ uint8_t smem_raw[];
+    constexpr bool SPLIT = FORM != WHOLE, PREFIX = FORM == PREFIXES;
     constexpr int HALVES = Geo<HD>::HALVES, Q_BYTES = Geo<HD>::Q_BYTES, KV_BYTES = Geo<HD>::KV_BYTES;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *q_s = smem;                       // [NT][Q_BYTES]
@@ -172,6 +178,7 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             mbar_init(BAR(sh.bar.o_done[t]), 1);
             for (int w = 0; w < 4; ++w) mbar_init(BAR(sh.bar.turn[w][t]), 1);
         }
+        if constexpr (PREFIX) mbar_init(BAR(sh.bar.v_tail), 1);
         fence_mbar_init();
         prefetch_tensormap(&tm_q);
         prefetch_tensormap(&tm_k);
@@ -201,13 +208,18 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int lane_base = 32 * (warp & 3);         // the TMEM lanes this warp may touch
     const int r = lane_base + lane;                // row of the tile
     int lo = a.tk, hi = 0;
-    const bool short_mask = a.mask.kind == 1 && a.tk <= OPEN_RUN_KEYS;
+    const bool short_mask = !PREFIX && a.mask.kind == 1 && a.tk <= OPEN_RUN_KEYS;
     if (warp >= 2 && warp < 2 + 4 * NT) {
         if (short_mask) {
             const OpenRun mine = open_run_share(a.mask, b, a.tk, sw);
             if (lane == 0) sh.open[sw] = mine;
         }
-        row_bounds_warp(a.mask, tile_row0(tile) + (r >> pack), a.tq, a.tk, lo, hi);
+        if constexpr (PREFIX) {
+            const int sequence = tile_row0(tile) + (r >> pack);
+            if (sequence < a.tq) prefix_bounds(a.reach, b, (int64_t)b * a.tq + sequence, lo, hi);
+        } else {
+            row_bounds_warp(a.mask, tile_row0(tile) + (r >> pack), a.tq, a.tk, lo, hi);
+        }
         int wlo = warp_min_i(hi > lo ? lo : a.tk), whi = warp_max_i(hi > lo ? hi : 0);
         if (lane == 0) { sh.red_lo[sw] = wlo; sh.red_hi[sw] = whi; }
     }
@@ -218,7 +230,7 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     int kmin = a.tk, kmax = 0;
 #pragma unroll
     for (int i = 0; i < 4 * NT; ++i) { kmin = min(kmin, sh.red_lo[i]); kmax = max(kmax, sh.red_hi[i]); }
-    bool padded = a.mask.kind == 1;   // there are flags to look at in the sweep
+    bool padded = !PREFIX && a.mask.kind == 1;   // there are flags to look at in the sweep
     const float rescale_at = hi - lo <= EXACT_KEYS ? 0.f : RESCALE_LOG2;   // (by what the row sees, padding or not)
     if (short_mask) {
         OpenRun run;
@@ -234,6 +246,8 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int subs = (!aborted && kmax > kmin) ? (kmax - kmin + SN - 1) / SN : 0;   // sub-steps of 64 keys
     const int steps = (subs + 1) / 2;                                                // K / V tiles of 128 keys
     bool failed = aborted;
+    const int v_rows = PREFIX ? kmax - kmin - (steps - 1) * BN : BN;   // rows of the last V tile that are there
+    const bool v_cut = PREFIX && v_rows < BN && kmax < a.tk;           // (past the tensor's end the copy brings zeros)
     // TMEM columns: S[tile][buffer] at 128 tile + 64 buffer (P over its first 32 columns), O[tile] at 256 + HD tile.
     auto COL_S = [](int t, int buf) { return static_cast<uint32_t>(t * BN + buf * SN); };
     auto COL_O = [](int t) { return static_cast<uint32_t>(256 + t * HD); };
@@ -260,6 +274,24 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 mbar_expect_tx(full, KV_BYTES);
 #pragma unroll
                 for (int half = 0; half < HALVES; ++half) tma_load_4d(dst + half * KV_HALF, &tm_v, full, 64 * half, hk, k0, b);
+            }
+        }
+        if constexpr (PREFIX) {
+            if (v_cut && steps > 0) {
+                const int st = (steps - 1) % NS, ph = ((steps - 1) / NS) & 1;
+                __syncwarp();   // (the tiles are asked for by lane 0)
+                const bool ok = __all_sync(0xffffffffu, mbar_wait(BAR(sh.bar.v_full[st]), ph));
+                if (ok) {
+                    for (int i = v_rows * 8 + lane; i < BN * 8; i += 32)
+#pragma unroll
+                        for (int half = 0; half < HALVES; ++half)
+                            reinterpret_cast<uint4 *>(v_s + st * KV_BYTES + half * KV_HALF)[i] = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(BAR(sh.bar.v_tail));
+                } else {
+                    failed = true;
+                }
             }
         }
     } else if (warp == MMA_WARP0 || warp == MMA_WARP1) {
@@ -306,6 +338,9 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 if (half == 0) {
                     ok = mbar_wait(FWD2_BAR(v_full) + 8 * st, i & 1) && ok;
                     if (more) ok = mbar_wait(FWD2_BAR(k_full) + 8 * (st ^ 1), (i + st) & 1) && ok;
+                    if constexpr (PREFIX) {
+                        if (v_cut && u >= subs - 2 + (subs & 1)) ok = mbar_wait(FWD2_BAR(v_tail), 0) && ok;   // the last tile
+                    }
                 }
                 if (!__all_sync(0xffffffffu, ok)) return false;
                 tc_fence_after_sync();
@@ -580,14 +615,24 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         tc_fence_after_sync();
         tmem_dealloc(tmem, 512);
     }
+    if constexpr (PREFIX) end_beside();
 }
 
 namespace {
 template <typename T, int HD>
+cudaError_t launch_fwd2_prefix_t(dim3 grid, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Sm100FwdArgs &a, bool beside,
+                                 cudaStream_t stream) {
+    constexpr size_t smem = Geo<HD>::SMEM_BYTES;
+    const auto kernel = fwd2_sm100_kernel<T, HD, PREFIXES>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    return launch_beside(kernel, grid, THREADS, smem, stream, beside, tq, tk, tv, tq, a);   // (no output map: it leaves parts)
+}
+template <typename T, int HD>
 cudaError_t launch_fwd2_t(dim3 grid, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const CUtensorMap &to,
                           const Sm100FwdArgs &a, cudaStream_t stream) {
     constexpr size_t smem = Geo<HD>::SMEM_BYTES;
-    const auto kernel = a.splits > 1 ? fwd2_sm100_kernel<T, HD, true> : fwd2_sm100_kernel<T, HD, false>;
+    const auto kernel = a.splits > 1 ? fwd2_sm100_kernel<T, HD, SPLITS> : fwd2_sm100_kernel<T, HD, WHOLE>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     kernel<<<grid, THREADS, smem, stream>>>(tq, tk, tv, to, a);
@@ -604,6 +649,17 @@ cudaError_t launch_fwd2_sm100(int dtype, const CUtensorMap &tq, const CUtensorMa
                          : launch_fwd2_t<__nv_bfloat16, 128>(grid, tq, tk, tv, to, a, stream);
     return a.d == 64 ? launch_fwd2_t<__half, 64>(grid, tq, tk, tv, to, a, stream)
                      : launch_fwd2_t<__half, 128>(grid, tq, tk, tv, to, a, stream);
+}
+
+cudaError_t launch_fwd2_prefix_sm100(int dtype, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Sm100FwdArgs &a,
+                                     bool beside, cudaStream_t stream) {
+    const int tokens = (NT * BM) >> a.pack;   // per block
+    dim3 grid(a.hq >> a.pack, (a.tq + tokens - 1) / tokens * a.splits, a.b);
+    if (dtype == DASH_ATTN_BF16)
+        return a.d == 64 ? launch_fwd2_prefix_t<__nv_bfloat16, 64>(grid, tq, tk, tv, a, beside, stream)
+                         : launch_fwd2_prefix_t<__nv_bfloat16, 128>(grid, tq, tk, tv, a, beside, stream);
+    return a.d == 64 ? launch_fwd2_prefix_t<__half, 64>(grid, tq, tk, tv, a, beside, stream)
+                     : launch_fwd2_prefix_t<__half, 128>(grid, tq, tk, tv, a, beside, stream);
 }
 
 cudaError_t read_sm100_fwd2_status(unsigned int *status, bool clear) {

@@ -65,6 +65,7 @@ constexpr int EXACT_KEYS = 512;
 struct Barriers {
     uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2];
     uint64_t s_full[2], s_empty[2], p_full[2], o_ready;
+    uint64_t v_tail;   // PREFIX: the rows of the last V tile that are past the prompt's end are zero
 };
 
 struct Shared {
@@ -94,11 +95,14 @@ template <> struct Pack<__half> {
 }  // namespace
 
 // SPLIT: the block sweeps one of a.splits runs of its tile's keys and leaves a part for the merge (as in the two-tile kernel).
-template <typename T, int HD, bool SPLIT>
+// PREFIX: split, over a decoding step's shared prompts (as in the two-tile kernel, values past a prompt's end cleared too).
+enum FwdForm { WHOLE, SPLITS, PREFIXES };
+template <typename T, int HD, FwdForm FORM>
 __global__ void __launch_bounds__(THREADS, 1)
 fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, const Sm100FwdArgs a) {
     extern __shared__ uint8_t smem_raw[];
+    constexpr bool SPLIT = FORM != WHOLE, PREFIX = FORM == PREFIXES;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     constexpr int PARTS = Geo1<HD>::PARTS, TILE_BYTES = Geo1<HD>::TILE_BYTES, NS = Geo1<HD>::NS;
     uint8_t *q_s = smem;
@@ -133,6 +137,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             mbar_init(BAR(sh.bar.p_full, i), 128);
         }
         mbar_init(o_ready, 1);
+        if constexpr (PREFIX) mbar_init(smem_u32(&sh.bar.v_tail), 1);
         fence_mbar_init();
         prefetch_tensormap(&tm_q);
         prefetch_tensormap(&tm_k);
@@ -149,7 +154,12 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     const int r = lane_base + lane;                // row of the tile (softmax threads)
     int lo = a.tk, hi = 0;
     if (warp >= 2 && warp < 6) {
-        row_bounds_warp(a.mask, m0 + (r >> pack), a.tq, a.tk, lo, hi);
+        if constexpr (PREFIX) {
+            const int sequence = m0 + (r >> pack);
+            if (sequence < a.tq) prefix_bounds(a.reach, b, (int64_t)b * a.tq + sequence, lo, hi);
+        } else {
+            row_bounds_warp(a.mask, m0 + (r >> pack), a.tq, a.tk, lo, hi);
+        }
         int wlo = warp_min_i(hi > lo ? lo : a.tk), whi = warp_max_i(hi > lo ? hi : 0);
         if (lane == 0) { sh.red_lo[sw] = wlo; sh.red_hi[sw] = whi; }
     }
@@ -160,13 +170,15 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     int kmin = a.tk, kmax = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) { kmin = min(kmin, sh.red_lo[i]); kmax = max(kmax, sh.red_hi[i]); }
-    if (a.mask.kind == 1) trim_padded(a.mask, b, kmin, kmax);
+    if (!PREFIX && a.mask.kind == 1) trim_padded(a.mask, b, kmin, kmax);
     if constexpr (SPLIT) split_keys(split, a.splits, BN, kmin, kmax);
     // Once a bounded wait has run out anywhere, later blocks do nothing: the call has failed and
     // the host will say so; there is no point in timing out thousands of times.
     const bool aborted = sh.abort != 0;
     const int n_tiles = (!aborted && kmax > kmin) ? (kmax - kmin + BN - 1) / BN : 0;
     bool failed = aborted;
+    const int v_rows = PREFIX ? kmax - kmin - (n_tiles - 1) * BN : BN;   // rows of the last V tile that are there
+    const bool v_cut = PREFIX && v_rows < BN && kmax < a.tk;             // (past the tensor's end the copy brings zeros)
 
     if (warp == 0) {
         // ---------------- TMA producer ----------------
@@ -196,6 +208,24 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                 for (int part = 0; part < PARTS; ++part) tma_load_4d(dst + part * HALF_BYTES, &tm_v, full, 64 * part, hk, k0, b);
             }
         }
+        if constexpr (PREFIX) {
+            if (v_cut && n_tiles > 0) {
+                const int st = (n_tiles - 1) % NS, ph = ((n_tiles - 1) / NS) & 1;
+                __syncwarp();   // (the tiles are asked for by lane 0)
+                const bool ok = __all_sync(0xffffffffu, mbar_wait(BAR(sh.bar.v_full, st), ph));
+                if (ok) {
+                    for (int i = v_rows * 8 + lane; i < BN * 8; i += 32)
+#pragma unroll
+                        for (int part = 0; part < PARTS; ++part)
+                            reinterpret_cast<uint4 *>(v_s + st * TILE_BYTES + part * HALF_BYTES)[i] = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&sh.bar.v_tail));
+                } else {
+                    failed = true;
+                }
+            }
+        }
     } else if (warp == 1) {
         // ---------------- MMA issuer: the whole warp runs the loop, one elected lane issues ----------------
         if (n_tiles > 0) {
@@ -207,6 +237,9 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                 const int vst = i % NS, vph = (i / NS) & 1;     // its V stage
                 if (!__all_sync(0xffffffffu, mbar_wait(BAR(sh.bar.v_full, vst), vph) && mbar_wait(BAR(sh.bar.p_full, st), ph)))
                     return false;
+                if constexpr (PREFIX) {
+                    if (v_cut && i == n_tiles - 1 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.bar.v_tail), 0))) return false;
+                }
                 tc_fence_after_sync();
                 // A = P: 16 keys = 32 bytes along the swizzled row, the second 64 keys in the second half.
                 // B = V: rows are keys (K of this product), 128 bytes of head dimension per row and half:
@@ -255,7 +288,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         // ---------------- softmax, one row per thread ----------------
         const int row = m0 + (r >> pack), h = h0 + (r & ((1 << pack) - 1));
         const uint32_t t_lane = tmem + (static_cast<uint32_t>(lane_base) << 16);
-        const bool padded = a.mask.kind == 1;
+        const bool padded = !PREFIX && a.mask.kind == 1;
         float m_ref = -INFINITY, l = 0.f;
         const float rescale_at = hi - lo <= EXACT_KEYS ? 0.f : RESCALE_LOG2;
         // The tile's 128 padding flags as four words; every warp gathers its own copy, so that no softmax
@@ -437,6 +470,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         tc_fence_after_sync();
         tmem_dealloc(tmem, 512);
     }
+    if constexpr (PREFIX) end_beside();
 }
 
 namespace {
@@ -444,13 +478,30 @@ template <typename T, int HD>
 cudaError_t launch_fwd_t(dim3 grid, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Sm100FwdArgs &a,
                          cudaStream_t stream) {
     constexpr size_t smem = Geo1<HD>::SMEM_BYTES;
-    const auto kernel = a.splits > 1 ? fwd_sm100_kernel<T, HD, HD == 256> : fwd_sm100_kernel<T, HD, false>;   // (D 128 here: a switch, never split)
+    const auto kernel = a.splits > 1 ? fwd_sm100_kernel<T, HD, HD == 256 ? SPLITS : WHOLE> : fwd_sm100_kernel<T, HD, WHOLE>;   // (D 128 here: a switch, never split)
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     kernel<<<grid, THREADS, smem, stream>>>(tq, tk, tv, a);
     return cudaGetLastError();
 }
+template <typename T>
+cudaError_t launch_fwd_prefix_t(dim3 grid, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Sm100FwdArgs &a, bool beside,
+                                cudaStream_t stream) {
+    constexpr size_t smem = Geo1<256>::SMEM_BYTES;
+    const auto kernel = fwd_sm100_kernel<T, 256, PREFIXES>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    return launch_beside(kernel, grid, THREADS, smem, stream, beside, tq, tk, tv, a);
+}
 }  // namespace
+
+cudaError_t launch_fwd_prefix_sm100(int dtype, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Sm100FwdArgs &a,
+                                    bool beside, cudaStream_t stream) {
+    const int tokens = BM >> a.pack;
+    dim3 grid(a.hq >> a.pack, (a.tq + tokens - 1) / tokens * a.splits, a.b);
+    return dtype == DASH_ATTN_BF16 ? launch_fwd_prefix_t<__nv_bfloat16>(grid, tq, tk, tv, a, beside, stream)
+                                   : launch_fwd_prefix_t<__half>(grid, tq, tk, tv, a, beside, stream);
+}
 
 cudaError_t launch_fwd_sm100(int dtype, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv,
                              const Sm100FwdArgs &a, cudaStream_t stream) {

@@ -13,6 +13,7 @@
 
 #include "common.cuh"
 #include "launch.h"
+#include "prefix.h"
 #include "sm100_kernels.h"
 
 namespace dash {
@@ -325,6 +326,56 @@ cudaError_t sm100_forward(const dash_attn_params *p, const TrainArgs &a, void *w
         *launches += 1;
     }
     return e;
+}
+
+// The prompts' part of a decoding step over shared prompts.  Runs of keys a tile of rows: as forward_splits estimates, but that there is
+// a merge whatever the number, and that a call of many tiles needs none.
+int sm100_prefix_splits(int dtype, float scale, int n, int each, int p, int hq, int hkv, int d) {
+    if (dtype == DASH_ATTN_F32 || (d != 64 && d != 128 && d != 256) || !(scale > 0.f) || !std::isfinite(scale)) return 0;
+    const bool one = d == 256;
+    const int pack = pack_log2(hq / hkv, each);
+    const int64_t sequences = (one ? 128 : 256) >> pack, step = one ? 128 : 64, sms = 148, tiles = (each + sequences - 1) / sequences;
+    if ((hq >> pack) > 65535 || n > 65535 || tiles > 65535) return 0;
+    const int64_t blocks = tiles * (hq >> pack) * n, l = (p + step - 1) / step, fixed = one ? 3 : 6;
+    const double part = (double)n * each * hq * d * sizeof(float) / (one ? 4.1e6 : 2.2e6);
+    auto cost = [&](int64_t s) { return (double)((blocks * s + sms - 1) / sms) * ((l + s - 1) / s + fixed) + s * part; };
+    int best = 1;
+    for (int s = 2; s <= 256 && s <= l && tiles * s <= 65535; ++s)
+        if (cost(s) < cost(best)) best = s;
+    return best;
+}
+bool sm100_prefix_takes(const PrefixArgs &a) {
+    // (A dimension that repeats, stride 0, has no tensor map.)
+    auto readable = [](const View4 &t, int n, int p, int h) {
+        const int64_t s[4] = {t.sb, t.st, t.sh, t.sd};
+        const int extent[3] = {n, p, h};
+        for (int i = 0; i < 3; ++i)
+            if (extent[i] > 1 && (s[i] <= 0 || s[i] >= (int64_t(1) << 39))) return false;
+        return tma_strides(s) && tma_base(t.ptr);
+    };
+    if (a.each > 1 && a.q_sb > (int64_t(1) << 39) / a.each) return false;
+    const View4 q{a.q, a.q_sb * a.each, a.q_sb, a.q_sh, a.q_sd};
+    return readable(q, a.n, a.each, a.hq) && readable(a.k, a.n, a.p, a.hkv) && readable(a.v, a.n, a.p, a.hkv) && device_is_sm100() && encoder();
+}
+bool sm100_prefix(int dtype, const PrefixArgs &a, bool beside, cudaStream_t stream, int *launches, cudaError_t *error) {
+    CUtensorMap tq, tk, tv;
+    const int pack = pack_log2(a.hq / a.hkv, a.each);
+    const int64_t qs[4] = {a.q_sb * a.each, a.q_sb, a.q_sh, a.q_sd}, ks[4] = {a.k.sb, a.k.st, a.k.sh, a.k.sd}, vs[4] = {a.v.sb, a.v.st, a.v.sh, a.v.sd};
+    if (!encode(&tq, dtype, a.q, a.n, a.each, a.hq, qs, 128, a.d, 1 << pack) || !encode(&tk, dtype, a.k.ptr, a.n, a.p, a.hkv, ks, 128, a.d) ||
+        !encode(&tv, dtype, a.v.ptr, a.n, a.p, a.hkv, vs, 128, a.d))
+        return false;
+    Sm100FwdArgs f{};
+    f.b = a.n; f.tq = a.each; f.tk = a.p; f.hq = a.hq; f.hkv = a.hkv; f.d = a.d;
+    f.scale = a.scale;
+    f.scale_log2 = a.scale * 1.4426950408889634f;
+    f.pack = pack;
+    f.splits = a.splits;
+    f.part_o = a.part_o;
+    f.part_lse = a.part_lse;
+    f.reach = a.reach;
+    *launches += 1;
+    *error = a.d == 256 ? launch_fwd_prefix_sm100(dtype, tq, tk, tv, f, beside, stream) : launch_fwd2_prefix_sm100(dtype, tq, tk, tv, f, beside, stream);
+    return true;
 }
 
 // Units that need no launch order: one a multiprocessor, at D 256 (two passes, two blocks to a unit) a quarter of that.  Units shared by two

@@ -22,6 +22,7 @@ struct Sm100FwdArgs {
     int splits;
     float *part_o;     // [splits][B,Tq,Hq,D]
     float *part_lse;   // [splits][B,Tq,Hq]
+    PrefixReach reach; // the prefix form: which keys of its prompt each sequence sees (the mask is not looked at)
 };
 
 // The run of a tile's keys [kmin, kmax) that falls to split `s`, in whole `step`s.
@@ -67,6 +68,12 @@ size_t bwd_sm100_fused_shared_bytes(int d);
 cudaError_t launch_fwd_merge(int dtype, const Sm100FwdArgs &a, cudaStream_t stream);
 cudaError_t launch_fwd_sm100(int dtype, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv,
                              const Sm100FwdArgs &a, cudaStream_t stream);
+// The prompts' part of a decoding step (prefix.cu): the forward's kernels over queries [N, sequences of a prompt, Hq, D] and keys
+// [N, P, Hkv, D], every block a part of its rows' keys.  `beside`: beside the launch in front of it.
+cudaError_t launch_fwd_prefix_sm100(int dtype, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Sm100FwdArgs &a,
+                                    bool beside, cudaStream_t stream);
+cudaError_t launch_fwd2_prefix_sm100(int dtype, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Sm100FwdArgs &a,
+                                     bool beside, cudaStream_t stream);
 // The two-tile forward: tq with boxes of 128 rows, tk / tv with boxes of 64 rows.
 cudaError_t launch_fwd2_sm100(int dtype, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv,
                               const CUtensorMap &to, const Sm100FwdArgs &a, cudaStream_t stream);

@@ -43,6 +43,22 @@ class Rope:
         self.cos = torch.from_numpy(cos).to(dtype).to(device)
         self.sin = torch.from_numpy(sin).to(dtype).to(device)
 
+    @classmethod
+    def from_tables(cls, cos: torch.Tensor, sin: torch.Tensor) -> "Rope":
+        """A rotation from tables that are there already, ``[len, dim]`` both, in the dtype of what they rotate: frequencies
+        that are scaled or spread otherwise than a base's powers.  The tables are kept, not copied."""
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.device != sin.device:
+            raise AttentionError(f"Rope: tables of {cos.dtype} {list(cos.shape)} and {sin.dtype} {list(sin.shape)}; [len, dim] both, one dtype and device")
+        dim = cos.shape[1]
+        if dim == 0 or dim % 2:
+            raise AttentionError(f"Rope: {dim} features; an even number is rotated")
+        if cos.dtype not in _DTYPES:
+            raise AttentionError(f"Rope: {cos.dtype} is not floating")
+        rope = cls.__new__(cls)
+        rope.dim, rope.base, rope._len, rope.dtype = dim, None, cos.shape[0], cos.dtype
+        rope.cos, rope.sin = cos.contiguous(), sin.contiguous()
+        return rope
+
     def len(self) -> int:
         """The last position this holds, plus one."""
         return self._len

@@ -9,12 +9,13 @@ from __future__ import annotations
 
 import ctypes
 import dataclasses
-from typing import Sequence
+from typing import Optional, Sequence
 
 import torch
 
 from . import _lib
 from .attention import AttentionError, _check_device, _DTYPES, _on, _ptr, _raise, _result, _stream, _workspace
+from .penalties import Penalties, penalize
 
 
 @dataclasses.dataclass(frozen=True)
@@ -62,8 +63,11 @@ def make_sample_params(logits: torch.Tensor, options: SampleOptions, token_dtype
     return p, ids
 
 
-def sample(logits: torch.Tensor, options: SampleOptions = SampleOptions(), token_dtype=torch.int64) -> Sampled:
-    """One token per row of ``logits [B, V]`` (crates/dash-ops/src/sample.rs ``sample``)."""
+def sample(logits: torch.Tensor, options: SampleOptions = SampleOptions(), token_dtype=torch.int64, penalties: Optional[Penalties] = None) -> Sampled:
+    """One token per row of ``logits [B, V]`` (crates/dash-ops/src/sample.rs ``sample``), of the logits under ``penalties`` where given;
+    the model's own log-probability is then the penalized logits' too."""
+    if penalties is not None:
+        logits = penalize(logits, penalties)
     if token_dtype == torch.int64:
         done = _lib.binding().sample(logits, options)
         if done is not None:

@@ -231,6 +231,99 @@ int dash_attn_decode_append_rope(const dash_attn_decode_params *p, const dash_ro
                                  dash_attn_stream_t stream);
 
 /*
+ * The norm of every query and key head with the rotation in the same pass: of each head's D features x,
+ *     y = R(n),   n = x / sqrt(mean(x^2) + eps) * weight,
+ * R the rotation of dash_rope_apply at the token's position.  The reference has no such form; here every step is f32 and a
+ * result rounds once (dash_rope_apply rounds its products, as the reference's whole-tensor form does).  Inputs
+ * [B, T, H, D] with any strides but contiguous features, read in place; outputs contiguous.  The position of token n = (b, t)
+ * is, first rule that applies: positions[n]; start + n - cu_seqlens[s] for the packed sequence s that holds n (tokens of no
+ * sequence pass through unchanged, neither normed nor rotated, and so do their gradients); start + t.  A range past the tables is
+ * refused; positions read on the device cannot be, and one outside the tables gives NaN in the rotated features.
+ */
+typedef struct dash_rope_norm_params {
+    int32_t b;
+    int64_t t;
+    int32_t d;                            /* up to 256 */
+    int32_t heads_q, heads_k;             /* heads_k = 0: one tensor */
+    int64_t q_stride[3], k_stride[3];     /* elements: batch, token, head */
+    int64_t grad_q_stride[3], grad_k_stride[3]; /* backward's other inputs (ignored by apply) */
+    int32_t weight_dtype;                 /* of the weights and of their gradients: the tensors' dtype or F32 */
+    float eps;
+    const void *positions;                /* [B * T] or NULL */
+    int32_t positions_elem_bytes;         /* 4 or 8 */
+    const void *cu_seqlens;               /* [cu_seqlens_len] or NULL; B = 1 */
+    int32_t cu_seqlens_len;
+    int32_t index_elem_bytes;             /* 4 or 8 */
+    int64_t start;
+} dash_rope_norm_params;
+
+/* weight_q, weight_k: [D] contiguous, or NULL: ones.  out_q may be q itself where q is contiguous, and out_k k. */
+int dash_rope_norm_apply(const dash_rope_tables *rope, const dash_rope_norm_params *p, const void *q, const void *k,
+                       const void *weight_q, const void *weight_k, void *out_q, void *out_k, dash_attn_stream_t stream);
+/* The gradients of q, k (contiguous, their dtype) and of the weights ([D], weight_dtype; NULL: not wanted) from those of out_q
+ * and out_k.  Nothing of the forward is needed but its inputs.  The weights' sums have a fixed order: the same bits on every run. */
+size_t dash_rope_norm_backward_workspace(const dash_rope_norm_params *p);
+int dash_rope_norm_backward(const dash_rope_tables *rope, const dash_rope_norm_params *p, const void *q, const void *k,
+                          const void *weight_q, const void *weight_k, const void *grad_q, const void *grad_k, void *dq, void *dk,
+                          void *dweight_q, void *dweight_k, void *workspace, size_t workspace_bytes, dash_attn_stream_t stream);
+
+/*
+ * The decoding step of a batch whose sequences share prompts: N prompts [N, P, Hkv, D], B = N * (sequences of a prompt), sequence
+ * b continuing prompt b / (B / N).  Its query sees the prompt's keys (of which the first lengths[n] are there) and, behind them,
+ * its own: the cache of dash_attn_decode_params, as in dash_attn_decode.  What dash_attn_decode gives on caches that hold the prompt's
+ * rows and then the sequence's own, with every prompt's rows held and read once for all of its sequences.  The window's left
+ * side counts over both.  k_new and v_new not NULL: the step appends, as dash_attn_decode_append does, to the sequence's own
+ * cache.  A sequence that sees no key gets zeros.
+ * What lies past a prompt's length, or past a sequence's, may be anything, NaN included.  (Under a window, keys of one prompt that
+ * some of its sequences see and others do not must be finite.)
+ */
+typedef struct dash_attn_prefix_params {
+    int32_t n, p;                           /* prompts, and the keys held for each; N divides B */
+    int32_t hkv, d, v_n, v_p, v_hkv, v_d;   /* the prompts' own dims, checked against the caches' and each other */
+    int64_t k_stride[4], v_stride[4];       /* elements: prompt, time, head, dim */
+    const void *lengths;                    /* [N] or NULL: every prompt has P keys */
+    int32_t lengths_len;                    /* must equal N when lengths != NULL */
+    int32_t lengths_elem_bytes;             /* 4 or 8 */
+} dash_attn_prefix_params;
+
+size_t dash_attn_decode_shared_workspace(const dash_attn_decode_params *p, const dash_attn_prefix_params *x);
+int dash_attn_decode_shared(const dash_attn_decode_params *p, const dash_attn_prefix_params *x, const void *q,
+                            const void *prefix_k, const void *prefix_v, const void *k_new, const void *v_new,
+                            void *k_cache, void *v_cache, void *out, void *workspace, size_t workspace_bytes,
+                            dash_attn_stream_t stream);
+
+/*
+ * The rules a server puts on a step's logits [B, V] before a token is drawn from them, per row:
+ *     seen[v]: v is among the row's history; count[v]: how often it is among the ids behind the prompt's;
+ *     z = seen[v] ? (z > 0 ? z / repetition : z * repetition) : z,
+ *     z = z - frequency * count[v] - presence * (count[v] > 0) + bias[v],
+ *     z = -inf where the grammar's bit of v is 0 (whatever it was, NaN included),
+ * in f32, rounded once to the logits' dtype.  Ids outside the vocabulary count for nothing (a padded history).  A row that is allowed
+ * nothing is -inf throughout.  dash_sample takes what comes out.
+ */
+typedef struct dash_sample_penalize_params {
+    int32_t dtype;                /* of the logits and of what comes out: DASH_ATTN_F32 / BF16 / F16 */
+    int32_t b, v;                 /* rows, vocabulary (up to 2^30) */
+    int64_t row_stride, out_stride; /* elements between rows; the vocabulary is contiguous */
+    const void *ids;              /* [B, ids_len] device memory, the prompt's ids and then the answer's; NULL: no history */
+    int32_t ids_len, ids_elem_bytes; /* 4 or 8 */
+    int64_t ids_stride;
+    const void *lengths;          /* [B] or NULL: how many ids each row holds (NULL: ids_len) */
+    const void *prompt_lengths;   /* [B] or NULL: how many of them are the prompt's (NULL: 0) */
+    int32_t lengths_elem_bytes, prompt_lengths_elem_bytes; /* 4 or 8 */
+    const float *repetition, *frequency, *presence; /* [B] device memory, or NULL: the value below for every row */
+    float repetition_all, frequency_all, presence_all; /* 1, 0, 0: no penalty.  repetition > 0 */
+    const void *bias;             /* [B, V] or (bias_stride 0) [V], or NULL */
+    int32_t bias_dtype;           /* the logits' dtype or F32 */
+    int64_t bias_stride;          /* elements between rows */
+    const void *allowed;          /* [B, ceil(V / 32)] 32-bit words, bit v % 32 of word v / 32, or NULL: every token */
+    int64_t allowed_stride;       /* words between rows; 0: one row for all */
+} dash_sample_penalize_params;
+
+/* out may be the logits themselves, with the same row stride. */
+int dash_sample_penalize(const dash_sample_penalize_params *p, const void *logits, void *out, dash_attn_stream_t stream);
+
+/*
  * Sampling the next token on the device, the step on the far side of the decoding loop: from the
  * logits [B, V] of one position per sequence, one token id per row with its log-probability under
  * the model's distribution, the model's at the temperature, and the one it was drawn from - the
