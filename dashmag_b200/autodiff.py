@@ -5,6 +5,8 @@ forward - its state is exactly ``(query, key, value, output, lse, mask, options)
 is the library's written-out backward pass, nothing is re-traced - and the routing of the decoding
 step when some input is tracked.  torch's autograd plays the part Burn's plays for the reference;
 every computation is still a call through the C ABI (``dashmag_b200.attention``).
+
+The norm of queries and keys with the rotation (``dashmag_b200.qk_norm``, not in the reference) is one node too, whose state is its inputs.
 """
 from __future__ import annotations
 
@@ -14,6 +16,7 @@ import torch
 
 from . import attention as A
 from .contract import AttentionMask, AttentionOptions
+from .qk_norm import QkNorm
 
 
 class AttentionNode(torch.autograd.Function):
@@ -102,3 +105,42 @@ def attention_decode(query, key, value, cache_lengths: Optional[torch.Tensor] = 
         output = AttentionNode.apply(query.reshape(b, 1, hq, d), key, value, AttentionMask.none(), options.with_causal(False))[0]
         return output.reshape(b, hq, d)
     return reference_decode(query, key, value, cache_lengths, options)
+
+
+class QkNormNode(torch.autograd.Function):
+    """The norm of a layer's query and key with the rotation: its state is the call's inputs, its backward the written-out pass."""
+
+    @staticmethod
+    def forward(ctx, query, key, query_weight, key_weight, norm: QkNorm, where: dict):
+        ctx.save_for_backward(query, key, query_weight, key_weight)
+        ctx.norm, ctx.where = norm, where
+        return norm._forward(query, key, where)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_query, grad_key):
+        query, key, query_weight, key_weight = ctx.saved_tensors
+        norm = QkNorm(ctx.norm.rope, query_weight, key_weight, ctx.norm.eps)
+        grads = norm._backward(query, key, grad_query, grad_key, ctx.where)
+        return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None)
+
+
+def _qk_norm(norm: QkNorm, query, key, where: dict):
+    if _tracked(*(t for t in (query, key, norm.query_weight, norm.key_weight) if t is not None)):
+        return QkNormNode.apply(query, key, norm.query_weight, norm.key_weight, norm, where)
+    return norm._forward(query, key, where)
+
+
+def qk_norm_range(norm: QkNorm, query, key, positions: range):
+    """``norm.apply_range`` for tensors and weights that may be tracked."""
+    return _qk_norm(norm, query, key, norm._range(query, key, positions))
+
+
+def qk_norm_at(norm: QkNorm, query, key, positions: torch.Tensor):
+    """``norm.apply_at`` for tensors and weights that may be tracked."""
+    return _qk_norm(norm, query, key, norm._at(query, key, positions))
+
+
+def qk_norm_packed(norm: QkNorm, query, key, cu_seqlens: torch.Tensor, start: int = 0):
+    """``norm.apply_packed`` for tensors and weights that may be tracked."""
+    return _qk_norm(norm, query, key, norm._packed(query, key, cu_seqlens, start))
