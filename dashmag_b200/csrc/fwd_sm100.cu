@@ -30,6 +30,7 @@
 
 #include "common.cuh"
 #include "sm100.h"
+#include "qk_norm.h"
 #include "sm100_kernels.h"
 #include "sm100_ptx.cuh"
 
@@ -527,7 +528,10 @@ cudaError_t read_sm100_status(unsigned int *status, bool clear) {
     e = read_sm100_bwd256_status(&bwd256, clear);
     if (e != cudaSuccess) return e;
     e = read_sm100_fwd2_status(&fwd2, clear);
-    *status |= bwd | fwd2 | bwd256;
+    if (e != cudaSuccess) return e;
+    unsigned int norm = 0;
+    e = read_qk_norm_status(&norm, clear);
+    *status |= bwd | fwd2 | bwd256 | norm;
     return e;
 }
 

@@ -21,6 +21,7 @@
 
 #include "common.cuh"
 #include "qk_norm.h"
+#include "sm100_ptx.cuh"
 
 namespace dash {
 namespace {
@@ -31,10 +32,30 @@ __device__ __forceinline__ int64_t index_at(const void *p, int bytes, int64_t i)
     return bytes == 8 ? static_cast<const int64_t *>(p)[i] : static_cast<int64_t>(static_cast<const int32_t *>(p)[i]);
 }
 
-// n = (batch element, token of it), in 32 bits where both fit.
+Over over_of(int64_t d) {   // (1 <= d < 2^31)
+    int l = 0;
+    while ((int64_t(1) << l) < d) ++l;
+    return Over{(uint32_t)((uint64_t(1) << 32) * ((uint64_t(1) << l) - d) / d + 1), l};
+}
+
+// What a warp of the ring kernel takes of one tensor at a time.
+struct RingPlan {
+    int heads, units;    // of a token; units of them to a token
+    int tokens;          // of a stage
+    int stage;           // bytes
+    Over over_heads;
+};
+
+// n / d for 0 <= n < 2^31 and d >= 1 by a multiplication (Granlund and Montgomery: m = floor(2^32 (2^l - d) / d) + 1, l = ceil(log2 d)).
+__device__ __forceinline__ uint32_t over(uint32_t n, const Over &o) { return (__umulhi(n, o.mul) + n) >> o.shift; }
+
+// n = (batch element, token of it).
 __device__ __forceinline__ void token_of(const NormArgs &a, int64_t n, int64_t &bi, int64_t &ti) {
-    if (((n | a.t) >> 32) == 0) {
-        bi = (uint32_t)n / (uint32_t)a.t;
+    bi = 0;
+    ti = n;
+    if (a.b == 1) return;
+    if (((n | a.t) >> 31) == 0) {
+        bi = over((uint32_t)n, a.over_t);
         ti = (uint32_t)n - (uint32_t)bi * (uint32_t)a.t;
     } else {
         bi = n / a.t;
@@ -42,26 +63,66 @@ __device__ __forceinline__ void token_of(const NormArgs &a, int64_t n, int64_t &
     }
 }
 
-// The position of token n = (.., ti): its row of the tables; -1 for one outside them, -2 for a token of no sequence.
-__device__ __forceinline__ int64_t table_row(const NormArgs &a, int64_t n, int64_t ti) {
+// The tokens [from, to) of the packed sequence that was found last (of no sequence where `held` is false): tokens are asked for in their
+// order, and most are of the sequence of the one before.
+struct Sequence {
+    int64_t from = 0, to = 0;
+    bool held = false;
+};
+
+// The position of token n = (.., ti): its row of the tables; -1 for one outside them, -2 for a token of no sequence.  Each lane for itself.
+__device__ __forceinline__ int64_t table_row(const NormArgs &a, int64_t n, int64_t ti, Sequence &seq) {
     int64_t pos;
     if (a.positions) {
         pos = index_at(a.positions, a.pos_bytes, n);
     } else if (a.cu) {
-        if (a.sequences <= 0 || n < index_at(a.cu, a.cu_bytes, 0) || n >= index_at(a.cu, a.cu_bytes, a.sequences)) return -2;
-        int lo = 0, hi = a.sequences;   // the last sequence whose offset is <= n
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (index_at(a.cu, a.cu_bytes, mid) <= n) lo = mid; else hi = mid;
+        if (n < seq.from || n >= seq.to) {
+            // The last offset that is <= n.
+            int lo = -1, hi = a.sequences + 1;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (index_at(a.cu, a.cu_bytes, mid) <= n) lo = mid; else hi = mid;
+            }
+            seq.held = lo >= 0 && lo < a.sequences;
+            seq.from = lo >= 0 ? index_at(a.cu, a.cu_bytes, lo) : 0;
+            seq.to = lo < a.sequences ? index_at(a.cu, a.cu_bytes, lo + 1) : 0x7fffffffffffffffLL;
         }
-        pos = a.start + n - index_at(a.cu, a.cu_bytes, lo);
+        if (!seq.held) return -2;
+        pos = a.start + n - seq.from;
     } else {
         pos = a.start + ti;
     }
     return pos >= 0 && pos < a.len ? pos : -1;
 }
+// The same where all 32 lanes ask for one token, once: each looks at one offset, 32 of them a look, so that a batch of up to 31 sequences
+// takes one trip to memory where the bisection takes one per step.
+__device__ __forceinline__ int64_t table_row_warp(const NormArgs &a, int64_t n, int64_t ti) {
+    int64_t pos;
+    if (!a.positions && a.cu) {
+        const int lane = threadIdx.x & 31;
+        int lo = 0, count = a.sequences + 1;   // among count offsets from lo on lies the last one that is <= n, if any
+        int64_t from = 0;
+        for (;;) {
+            const int hop = (count + 31) / 32, mine = lo + lane * hop;
+            const int64_t offset = mine < lo + count ? index_at(a.cu, a.cu_bytes, mine) : 0x7fffffffffffffffLL;
+            const unsigned below = __ballot_sync(0xffffffffu, offset <= n);
+            if (below == 0) return -2;   // (only at the first look: before the first offset)
+            const int last = 31 - __clz(below);
+            from = __shfl_sync(0xffffffffu, offset, last);
+            count = min(hop, count - last * hop);
+            lo += last * hop;
+            if (hop == 1) break;
+        }
+        if (lo >= a.sequences) return -2;   // behind the last offset
+        pos = a.start + n - from;
+    } else {
+        pos = a.positions ? index_at(a.positions, a.pos_bytes, n) : a.start + ti;
+    }
+    return pos >= 0 && pos < a.len ? pos : -1;
+}
 
-// V elements of T as they lie in memory, 16 bytes (weights in f32 beside 16-bit tensors: 32).
+// V elements of T as they lie in memory, 16 bytes (weights in f32 beside 16-bit tensors: 32), and as pairs of f32, two to a
+// packed instruction.
 template <typename T, int V> struct alignas(16) Vec { T e[V]; };
 template <typename T, int V> __device__ __forceinline__ Vec<T, V> load(const T *p) {
     Vec<T, V> v;
@@ -72,21 +133,16 @@ template <typename T, int V> __device__ __forceinline__ Vec<T, V> load(const T *
 template <typename T, int V> __device__ __forceinline__ void store(T *p, const Vec<T, V> &v) {
     *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(&v);
 }
-template <typename T, int V> __device__ __forceinline__ void widen(const Vec<T, V> &v, float (&x)[V]) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) x[e] = Num<T>::to_f32(v.e[e]);
+template <int V> __device__ __forceinline__ float2 pair(const Vec<float, V> &v, int i) { return make_float2(v.e[2 * i], v.e[2 * i + 1]); }
+template <int V> __device__ __forceinline__ float2 pair(const Vec<__nv_bfloat16, V> &v, int i) {
+    const uint32_t u = reinterpret_cast<const uint32_t *>(&v)[i];
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
-template <typename T, int V> __device__ __forceinline__ Vec<T, V> narrow(const float (&x)[V]) {
-    Vec<T, V> v;
-#pragma unroll
-    for (int e = 0; e < V; ++e) v.e[e] = Num<T>::from_f32(x[e]);
-    return v;
-}
-template <typename TW, int V> __device__ __forceinline__ void weights(const void *w, int col, bool live, float (&x)[V]) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) x[e] = 1.f;
-    if (w && live) widen<TW, V>(load<TW, V>(static_cast<const TW *>(w) + col), x);
-}
+template <int V> __device__ __forceinline__ float2 pair(const Vec<__half, V> &v, int i) { return __half22float2(reinterpret_cast<const __half2 *>(&v)[i]); }
+template <int V> __device__ __forceinline__ void put(Vec<float, V> &v, int i, float2 x) { v.e[2 * i] = x.x; v.e[2 * i + 1] = x.y; }
+template <int V> __device__ __forceinline__ void put(Vec<__nv_bfloat16, V> &v, int i, float2 x) { reinterpret_cast<__nv_bfloat162 *>(&v)[i] = __float22bfloat162_rn(x); }
+template <int V> __device__ __forceinline__ void put(Vec<__half, V> &v, int i, float2 x) { reinterpret_cast<__half2 *>(&v)[i] = __float22half2_rn(x); }
+
 template <int LPH> __device__ __forceinline__ float head_sum(float x) {
 #pragma unroll
     for (int o = LPH / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
@@ -94,24 +150,8 @@ template <int LPH> __device__ __forceinline__ float head_sum(float x) {
 }
 
 __device__ __forceinline__ float nan_f32() { return __int_as_float(0x7fc00000); }
-
-// Cosines and sines of a lane's two columns: the token's row, NaN for a position outside the tables (nothing is read there), and no
-// rotation for columns behind the rotated ones.
-template <typename T, int V> struct Turn {
-    float c1[V], c2[V], s1[V], s2[V];
-    __device__ __forceinline__ Turn(const NormArgs &a, int64_t row, bool rotated, int c, int half) {
-        const float none = rotated ? nan_f32() : 1.f, off = rotated ? none : 0.f;
-#pragma unroll
-        for (int e = 0; e < V; ++e) { c1[e] = c2[e] = none; s1[e] = s2[e] = off; }
-        if (rotated && row >= 0) {
-            const T *cs = static_cast<const T *>(a.cos) + row * a.dim + c, *sn = static_cast<const T *>(a.sin) + row * a.dim + c;
-            widen<T, V>(load<T, V>(cs), c1);
-            widen<T, V>(load<T, V>(cs + half), c2);
-            widen<T, V>(load<T, V>(sn), s1);
-            widen<T, V>(load<T, V>(sn + half), s2);
-        }
-    }
-};
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 neg2(float2 x) { return make_float2(-x.x, -x.y); }
 
 // A lane's place in a head of the vector kernels.
 template <int V, int LPH> struct Place {
@@ -126,13 +166,47 @@ template <int V, int LPH> struct Place {
     }
 };
 
+// The weights of a lane's columns, as they lie in memory; ones where there are none.
+template <typename TW, int V, int LPH> struct Weights {
+    Vec<TW, V> w1, w2;
+    __device__ __forceinline__ Weights(const void *w, const Place<V, LPH> &at) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) w1.e[e] = w2.e[e] = Num<TW>::from_f32(1.f);
+        if (w && at.live) {
+            w1 = load<TW, V>(static_cast<const TW *>(w) + at.c1);
+            w2 = load<TW, V>(static_cast<const TW *>(w) + at.c2);
+        }
+    }
+};
+
+// Cosines and sines of a lane's columns, as they lie in memory: the token's row; NaN for a position outside the tables (nothing is read there);
+// no rotation for columns behind the rotated ones.
+template <typename T, int V, int LPH> struct Turn {
+    Vec<T, V> c1, c2, s1, s2;
+    __device__ __forceinline__ Turn(const NormArgs &a, int64_t row, const Place<V, LPH> &at) {
+        const bool turned = at.live && at.rotated;
+        if (turned && row >= 0) {
+            const T *cs = static_cast<const T *>(a.cos) + row * a.dim + at.c1, *sn = static_cast<const T *>(a.sin) + row * a.dim + at.c1;
+            c1 = load<T, V>(cs);
+            c2 = load<T, V>(cs + a.dim / 2);
+            s1 = load<T, V>(sn);
+            s2 = load<T, V>(sn + a.dim / 2);
+        } else {
+            const T c = Num<T>::from_f32(turned ? nan_f32() : 1.f), s = Num<T>::from_f32(turned ? nan_f32() : 0.f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) { c1.e[e] = c2.e[e] = c; s1.e[e] = s2.e[e] = s; }
+        }
+    }
+};
+
+// The weight is multiplied into the token's cosines and sines, once for all heads of the lane: y1 = r (x1 w1 c1 - x2 w2 s1) and
+// y2 = r (x2 w2 c2 + x1 w1 s2) are then two products and two sums a column.
 template <typename T, typename TW, int V, int LPH, int HG>
-__global__ void __launch_bounds__(THREADS) qk_norm_kernel(NormArgs a, int units_q, int units_k) {
+__global__ void __launch_bounds__(THREADS) qk_norm_kernel(NormArgs a, int units_q, int units, Over over_units) {
     constexpr int NG = 32 / LPH;   // heads of a warp's load
     const int lane = threadIdx.x & 31;
     const int64_t warp = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-    const int units = units_q + units_k;
-    const int64_t n = (warp >> 31) == 0 ? (int64_t)((uint32_t)warp / (uint32_t)units) : warp / units;
+    const int64_t n = (warp >> 31) == 0 ? (int64_t)over((uint32_t)warp, over_units) : warp / units;
     if (n >= a.b * a.t) return;
     const int unit = (int)(warp - n * units);
     const bool is_k = unit >= units_q;
@@ -141,154 +215,296 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(NormArgs a, int units_
     const Place<V, LPH> at(a, lane);
     int64_t bi, ti;
     token_of(a, n, bi, ti);
-    const T *x = static_cast<const T *>(t.x) + bi * t.sb + ti * t.st;
-    T *out = static_cast<T *>(t.out) + n * t.heads * a.d;
+    const int64_t hop = NG * t.sh;
+    const T *x = static_cast<const T *>(t.x) + bi * t.sb + ti * t.st + h0 * t.sh + at.c1;
+    T *out = static_cast<T *>(t.out) + (n * t.heads + h0) * a.d + at.c1;
+    const int other = at.c2 - at.c1;
     Vec<T, V> x1[HG], x2[HG];
 #pragma unroll
     for (int g = 0; g < HG; ++g) {
-        const int h = min(h0 + g * NG, t.heads - 1);
-        if (at.live) {
-            x1[g] = load<T, V>(x + h * t.sh + at.c1);
-            x2[g] = load<T, V>(x + h * t.sh + at.c2);
+        if (at.live && h0 + g * NG < t.heads) {
+            x1[g] = load<T, V>(x + g * hop);
+            x2[g] = load<T, V>(x + g * hop + other);
         }
     }
-    float w1[V], w2[V];
-    weights<TW, V>(t.w, at.c1, at.live, w1);
-    weights<TW, V>(t.w, at.c2, at.live, w2);
-    const int64_t row = table_row(a, n, ti);
-    const Turn<T, V> turn(a, row, at.live && at.rotated, at.c1, a.dim / 2);
+    const Weights<TW, V, LPH> w(t.w, at);
+    const int64_t row = table_row_warp(a, n, ti);
+    float2 k1[V / 2], k2[V / 2], z1[V / 2], z2[V / 2];   // w1 c1, w2 c2, -w2 s1, w1 s2
+    {
+        const Turn<T, V, LPH> turn(a, row, at);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            k1[i] = ptx::mul2(pair<V>(w.w1, i), pair<V>(turn.c1, i));
+            k2[i] = ptx::mul2(pair<V>(w.w2, i), pair<V>(turn.c2, i));
+            z1[i] = neg2(ptx::mul2(pair<V>(w.w2, i), pair<V>(turn.s1, i)));
+            z2[i] = ptx::mul2(pair<V>(w.w1, i), pair<V>(turn.s2, i));
+        }
+    }
+    const float inv_d = 1.f / a.d;
 #pragma unroll
     for (int g = 0; g < HG; ++g) {
-        const int h = h0 + g * NG;
-        float u1[V], u2[V], sum = 0.f;
-        if (at.live) {
-            widen<T, V>(x1[g], u1);
-            widen<T, V>(x2[g], u2);
+        const bool live = at.live && h0 + g * NG < t.heads;
+        float2 u1[V / 2], u2[V / 2], sum = both(0.f);
+        if (live) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) sum = fmaf(u1[e], u1[e], fmaf(u2[e], u2[e], sum));
-        }
-        const float r = rsqrtf(head_sum<LPH>(sum) / a.d + a.eps);
-        if (!at.live || h >= t.heads) continue;
-        Vec<T, V> y1 = x1[g], y2 = x2[g];
-        if (row != -2) {   // (a token of no sequence passes unchanged)
-            float z1[V], z2[V];
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float n1 = u1[e] * r * w1[e], n2 = u2[e] * r * w2[e];
-                z1[e] = n1 * turn.c1[e] - n2 * turn.s1[e];
-                z2[e] = n2 * turn.c2[e] + n1 * turn.s2[e];
+            for (int i = 0; i < V / 2; ++i) {
+                u1[i] = pair<V>(x1[g], i);
+                u2[i] = pair<V>(x2[g], i);
+                sum = ptx::fma2(u1[i], u1[i], ptx::fma2(u2[i], u2[i], sum));
             }
-            y1 = narrow<T, V>(z1);
-            y2 = narrow<T, V>(z2);
         }
-        store<T, V>(out + h * a.d + at.c1, y1);
-        store<T, V>(out + h * a.d + at.c2, y2);
+        const float r = rsqrtf(fmaf(head_sum<LPH>(sum.x + sum.y), inv_d, a.eps));
+        if (!live) continue;
+        if (row != -2) {   // (a token of no sequence passes unchanged)
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                put<V>(x1[g], i, ptx::mul2(ptx::fma2(u1[i], k1[i], ptx::mul2(u2[i], z1[i])), both(r)));
+                put<V>(x2[g], i, ptx::mul2(ptx::fma2(u2[i], k2[i], ptx::mul2(u1[i], z2[i])), both(r)));
+            }
+        }
+        store<T, V>(out + g * NG * a.d, x1[g]);
+        store<T, V>(out + g * NG * a.d + other, x2[g]);
     }
 }
 
 // A block's sums of the weight's gradient, from its warps' lanes, into its row of the scratch.
-template <int V, int LPH>
-__device__ __forceinline__ void leave_part(const NormArgs &a, const Place<V, LPH> &at, float (&d1)[V], float (&d2)[V], float *red) {
+template <int V, int LPH, int NW>
+__device__ __forceinline__ void leave_part(const NormArgs &a, const Place<V, LPH> &at, const float2 (&d1)[V / 2], const float2 (&d2)[V / 2], float *red) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
+        float u1 = e & 1 ? d1[e / 2].y : d1[e / 2].x, u2 = e & 1 ? d2[e / 2].y : d2[e / 2].x;
 #pragma unroll
         for (int o = LPH; o < 32; o <<= 1) {
-            d1[e] += __shfl_xor_sync(0xffffffffu, d1[e], o);
-            d2[e] += __shfl_xor_sync(0xffffffffu, d2[e], o);
+            u1 += __shfl_xor_sync(0xffffffffu, u1, o);
+            u2 += __shfl_xor_sync(0xffffffffu, u2, o);
         }
         if (lane < LPH && at.live) {
-            red[warp * a.d + at.c1 + e] = d1[e];
-            red[warp * a.d + at.c2 + e] = d2[e];
+            red[warp * a.d + at.c1 + e] = u1;
+            red[warp * a.d + at.c2 + e] = u2;
         }
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < a.d; c += THREADS) {
+    for (int c = threadIdx.x; c < a.d; c += NW * 32) {
         float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < WARPS; ++i) sum += red[i * a.d + c];
+        for (int i = 0; i < NW; ++i) sum += red[i * a.d + c];
         a.part[(int64_t)blockIdx.x * a.d + c] = sum;
     }
 }
 
-// The blocks up to blocks_q take the queries' units in turn, the others the keys', so that a lane's sums of the weight's gradient
-// are one tensor's and stay in registers to the end.
-template <typename T, typename TW, int V, int LPH, int HG>
-__global__ void __launch_bounds__(THREADS) qk_norm_backward_kernel(NormArgs a, int units_q, int units_k, int blocks_q) {
-    constexpr int NG = 32 / LPH;
-    extern __shared__ float red[];   // [WARPS][d]
-    allow_beside();   // the sums over the blocks
-    const int lane = threadIdx.x & 31;
-    const bool is_k = (int)blockIdx.x >= blocks_q;
-    const NormTensor &t = is_k ? a.k : a.q;
-    const int units = is_k ? units_k : units_q;
-    const int64_t first = (int64_t)(is_k ? blockIdx.x - blocks_q : blockIdx.x) * WARPS + (threadIdx.x >> 5);
-    const int64_t step = (int64_t)(is_k ? gridDim.x - blocks_q : blocks_q) * WARPS, all = a.b * a.t * units;
-    const Place<V, LPH> at(a, lane);
-    float w1[V], w2[V], d1[V], d2[V];
-    weights<TW, V>(t.w, at.c1, at.live, w1);
-    weights<TW, V>(t.w, at.c2, at.live, w2);
+// ---------------------------------------------------------------------------------------------
+// Calls of many tokens, and the gradient
+// ---------------------------------------------------------------------------------------------
+// The blocks up to blocks_q take the queries, the others the keys; a warp takes the same heads of one token after another, or, where a
+// token's heads are few, all heads of several tokens at a time.  What it needs of a token - its heads, the gradient of them, the token's
+// row of the tables - comes as whole runs of bytes, each asked for by one lane, into a ring of two stages of shared memory of the
+// warp's own: the tokens behind the ones it works on are on their way meanwhile at the price of neither registers nor instructions, and
+// the warps of a block know nothing of one another.
+// The weight's gradient: a lane's sums are one tensor's columns and stay in registers to the end.
+__device__ unsigned int g_qk_norm_status = 0;   // sticky: non-zero once a bounded wait has run out
+
+// Of a stage: HG loads of 32 / LPH heads each.  Four warps a block and three blocks a multiprocessor: 168 registers, with which nothing spills.
+template <bool BACK> struct Ring {
+    static constexpr int HG = BACK ? 4 : 8, STAGES = 2, WARPS = 4, BLOCKS = 3;
+};
+constexpr int STAGE_MOST = 9216;   // bytes: three blocks of four warps of two fill a multiprocessor's shared memory
+constexpr int stage_bytes(bool back, int heads, int tokens, int d, int dim, int eb) { return (heads * d * (back ? 2 : 1) + tokens * 2 * dim) * eb; }
+
+// `heads` of a token, `sh` elements apart: one run where they lie side by side, else one each.
+template <typename T>
+__device__ __forceinline__ void heads_load(const NormArgs &a, const T *x, int64_t sh, int heads, uint32_t to, uint32_t bar) {
+    const int size = a.d * (int)sizeof(T);
+    if (sh == a.d) {
+        ptx::bulk_load(to, x, heads * size, bar);
+    } else {
+        for (int h = 0; h < heads; ++h) ptx::bulk_load(to + h * size, x + h * sh, size, bar);
+    }
+}
+
+// A lane's cosines and sines as f32 pairs; forward the weight is multiplied in, once for all heads of a token:
+// y1 = r (x1 k1 + x2 z1), y2 = r (x2 k2 + x1 z2) with k1 = w1 c1, k2 = w2 c2, z1 = -w2 s1, z2 = w1 s2; backward c1, c2, -s1, s2.
+// `kind` 0: the row is there; else NaN.  Columns behind the rotated ones: no rotation.
+template <typename T, typename TW, int V, int LPH, bool BACK>
+struct Factors {
+    float2 k1[V / 2], k2[V / 2], z1[V / 2], z2[V / 2];
+    __device__ __forceinline__ void set(const T *row, int dim, const Place<V, LPH> &at, const Weights<TW, V, LPH> &w, unsigned kind) {
+        Vec<T, V> c1, c2, s1, s2;
+        const bool turned = at.live && at.rotated;
+        if (turned && kind == 0) {
+            c1 = load<T, V>(row + at.c1);
+            c2 = load<T, V>(row + at.c2);
+            s1 = load<T, V>(row + dim + at.c1);
+            s2 = load<T, V>(row + dim + at.c2);
+        } else {
+            const T c = Num<T>::from_f32(turned ? nan_f32() : 1.f), z = Num<T>::from_f32(turned ? nan_f32() : 0.f);
 #pragma unroll
-    for (int e = 0; e < V; ++e) d1[e] = d2[e] = 0.f;
-    for (int64_t item = first; item < all; item += step) {
-        const int64_t n = (item >> 31) == 0 ? (int64_t)((uint32_t)item / (uint32_t)units) : item / units;
-        const int h0 = (int)(item - n * units) * NG * HG + lane / LPH;
-        int64_t bi, ti;
-        token_of(a, n, bi, ti);
-        const T *x = static_cast<const T *>(t.x) + bi * t.sb + ti * t.st, *dy = static_cast<const T *>(t.g) + bi * t.gb + ti * t.gt;
-        T *out = static_cast<T *>(t.out) + n * t.heads * a.d;
-        Vec<T, V> x1[HG], x2[HG], y1[HG], y2[HG];
-#pragma unroll
-        for (int g = 0; g < HG; ++g) {
-            const int h = min(h0 + g * NG, t.heads - 1);
-            if (at.live) {
-                x1[g] = load<T, V>(x + h * t.sh + at.c1);
-                x2[g] = load<T, V>(x + h * t.sh + at.c2);
-                y1[g] = load<T, V>(dy + h * t.gh + at.c1);
-                y2[g] = load<T, V>(dy + h * t.gh + at.c2);
-            }
+            for (int e = 0; e < V; ++e) { c1.e[e] = c2.e[e] = c; s1.e[e] = s2.e[e] = z; }
         }
-        const int64_t row = table_row(a, n, ti);
-        const Turn<T, V> turn(a, row, at.live && at.rotated, at.c1, a.dim / 2);
 #pragma unroll
-        for (int g = 0; g < HG; ++g) {
-            const int h = h0 + g * NG;
-            float u1[V], u2[V], g1[V], g2[V], square = 0.f, along = 0.f;
-            if (at.live) {
-                float v1[V], v2[V];
-                widen<T, V>(x1[g], u1);
-                widen<T, V>(x2[g], u2);
-                widen<T, V>(y1[g], v1);
-                widen<T, V>(y2[g], v2);
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    g1[e] = v1[e] * turn.c1[e] + v2[e] * turn.s2[e];
-                    g2[e] = v2[e] * turn.c2[e] - v1[e] * turn.s1[e];
-                    square = fmaf(u1[e], u1[e], fmaf(u2[e], u2[e], square));
-                    along = fmaf(u1[e] * w1[e], g1[e], fmaf(u2[e] * w2[e], g2[e], along));
-                }
+        for (int i = 0; i < V / 2; ++i) {
+            k1[i] = pair<V>(c1, i);
+            k2[i] = pair<V>(c2, i);
+            z1[i] = neg2(pair<V>(s1, i));
+            z2[i] = pair<V>(s2, i);
+            if constexpr (!BACK) {
+                const float2 w1 = pair<V>(w.w1, i), w2 = pair<V>(w.w2, i);
+                k1[i] = ptx::mul2(k1[i], w1);
+                k2[i] = ptx::mul2(k2[i], w2);
+                z1[i] = ptx::mul2(z1[i], w2);
+                z2[i] = ptx::mul2(z2[i], w1);
             }
-            const float r = rsqrtf(head_sum<LPH>(square) / a.d + a.eps);
-            const float back = head_sum<LPH>(along) / a.d * r * r * r;
-            if (!at.live || h >= t.heads) continue;
-            Vec<T, V> z1 = y1[g], z2 = y2[g];
-            if (row != -2) {
-                float e1[V], e2[V];
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    e1[e] = r * w1[e] * g1[e] - u1[e] * back;
-                    e2[e] = r * w2[e] * g2[e] - u2[e] * back;
-                    d1[e] = fmaf(g1[e], u1[e] * r, d1[e]);
-                    d2[e] = fmaf(g2[e], u2[e] * r, d2[e]);
-                }
-                z1 = narrow<T, V>(e1);
-                z2 = narrow<T, V>(e2);
-            }
-            store<T, V>(out + h * a.d + at.c1, z1);
-            store<T, V>(out + h * a.d + at.c2, z2);
         }
     }
-    leave_part<V, LPH>(a, at, d1, d2, red);
+};
+
+template <typename T, typename TW, int V, int LPH, bool BACK>
+__global__ void __launch_bounds__(Ring<BACK>::WARPS * 32, Ring<BACK>::BLOCKS) qk_norm_ring_kernel(NormArgs a, RingPlan of_q, RingPlan of_k, int blocks_q) {
+    using R = Ring<BACK>;
+    constexpr int NG = 32 / LPH, STAGES = R::STAGES, NW = R::WARPS;
+    extern __shared__ __align__(128) uint8_t smem[];   // barriers [NW][STAGES], rings [NW][STAGES][stage]; at the end the sums [NW][d]
+    if constexpr (BACK) allow_beside();   // the sums over the blocks
+    const int lane = threadIdx.x & 31, wib = threadIdx.x >> 5;
+    const bool is_k = (int)blockIdx.x >= blocks_q;
+    const NormTensor &t = is_k ? a.k : a.q;
+    const RingPlan &plan = is_k ? of_k : of_q;
+    const int units = plan.units, each = plan.tokens;
+    const bool many = each > 1;
+    const int row_size = a.dim * (int)sizeof(T), head_size = a.d * (int)sizeof(T);
+    const int xs_at = each * 2 * row_size, ys_at = xs_at + plan.heads * each * head_size;   // in a stage: the tables' rows, x, the gradients
+    uint8_t *mine = smem + 128 + wib * STAGES * plan.stage;
+    const uint32_t mine_u32 = ptx::smem_u32(mine), bars = ptx::smem_u32(smem) + wib * STAGES * 8;
+    if (lane == 0) {
+        for (int s = 0; s < STAGES; ++s) ptx::mbar_init(bars + 8 * s, many ? 32 : 1);
+        ptx::fence_mbar_init();
+    }
+    __syncwarp();
+    // Warps in whole sets of `units`; what is left over (fewer than `units`) stands by.  (More units than warps: one set, in rounds.)
+    const int warps = (is_k ? gridDim.x - blocks_q : blocks_q) * NW, number = (is_k ? blockIdx.x - blocks_q : blockIdx.x) * NW + wib;
+    const int sets = max(warps / units, 1), set = warps >= units ? number / units : 0;
+    const int64_t tokens = set < sets && *reinterpret_cast<volatile unsigned int *>(&g_qk_norm_status) == 0 ? a.b * a.t : 0;
+    const int64_t first = (int64_t)set * each, step = (int64_t)sets * each;
+    const Place<V, LPH> at(a, lane);
+    const Weights<TW, V, LPH> w(t.w, at);
+    const float inv_d = 1.f / a.d;
+    float2 d1[V / 2], d2[V / 2];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) d1[i] = d2[i] = both(0.f);
+    unsigned phase = 0, pending = 0;   // bit per stage: the parity waited for next; whether its copies have been asked for and not met
+    bool failed = false;
+    for (int unit = number - set * units; unit < units && !failed; unit += warps >= units ? units : warps) {
+        const int h0 = unit * plan.heads, heads = min(plan.heads, t.heads - h0);
+        unsigned what = 0;   // two bits per stage, of this lane's token: 0 a row of the tables is there, 1 the position is outside them, 2 a token of no sequence
+        Sequence seq;
+        // The tokens from n on into stage s: lane i asks for the i-th of them.
+        auto ask = [&](int64_t n, int s) {
+            if (n >= tokens) return;
+            pending |= 1u << s;
+            if (!many && lane != 0) return;
+            const uint32_t bar = bars + 8 * s, to = mine_u32 + s * plan.stage;
+            n += lane;
+            if (lane >= each || n >= tokens) {
+                ptx::mbar_arrive(bar);
+                return;
+            }
+            int64_t bi, ti;
+            token_of(a, n, bi, ti);
+            const int64_t row = table_row(a, n, ti, seq);
+            what = (what & ~(3u << (2 * s))) | ((unsigned)(row >= 0 ? 0 : -row) << (2 * s));
+            ptx::mbar_expect_tx(bar, (BACK ? 2 : 1) * heads * head_size + (row >= 0 ? 2 * row_size : 0));
+            if (row >= 0) {
+                ptx::bulk_load(to + lane * 2 * row_size, static_cast<const T *>(a.cos) + row * a.dim, row_size, bar);
+                ptx::bulk_load(to + lane * 2 * row_size + row_size, static_cast<const T *>(a.sin) + row * a.dim, row_size, bar);
+            }
+            heads_load<T>(a, static_cast<const T *>(t.x) + bi * t.sb + ti * t.st + h0 * t.sh, t.sh, heads, to + xs_at + lane * heads * head_size, bar);
+            if constexpr (BACK)
+                heads_load<T>(a, static_cast<const T *>(t.g) + bi * t.gb + ti * t.gt + h0 * t.gh, t.gh, heads, to + ys_at + lane * heads * head_size, bar);
+        };
+        ask(first, 0);
+        int s = 0;
+        for (int64_t n = first; n < tokens; n += step) {
+            __syncwarp();   // (the stage that is asked for next has been read by every lane)
+            ask(n + step, s ^ 1);
+            __syncwarp();
+            if (!__all_sync(0xffffffffu, ptx::mbar_wait(bars + 8 * s, phase >> s & 1u))) { failed = true; break; }
+            phase ^= 1u << s;
+            pending &= ~(1u << s);
+            const uint8_t *stage = mine + s * plan.stage;
+            const T *xs = reinterpret_cast<const T *>(stage + xs_at), *ys = reinterpret_cast<const T *>(stage + ys_at);
+            T *out = static_cast<T *>(t.out) + (n * t.heads + h0) * a.d;
+            const unsigned kinds = what >> (2 * s) & 3u;
+            unsigned kind = __shfl_sync(0xffffffffu, kinds, 0);
+            Factors<T, TW, V, LPH, BACK> f;
+            if (!many) f.set(reinterpret_cast<const T *>(stage), a.dim, at, w, kind);
+            const int rows = (int)min((int64_t)each, tokens - n) * heads;
+#pragma unroll 2
+            for (int r0 = 0; r0 < rows; r0 += NG) {
+                const int row = r0 + lane / LPH;   // the head, of the stage's all
+                const bool live = at.live && row < rows;
+                if (many) {
+                    const int token = min((int)over((uint32_t)row, plan.over_heads), each - 1);
+                    kind = __shfl_sync(0xffffffffu, kinds, token);
+                    f.set(reinterpret_cast<const T *>(stage + token * 2 * row_size), a.dim, at, w, kind);
+                }
+                float2 u1[V / 2], u2[V / 2], g1[V / 2], g2[V / 2], square = both(0.f), along = both(0.f);
+                Vec<T, V> y1, y2;
+                if (live) {
+                    const Vec<T, V> x1 = load<T, V>(xs + row * a.d + at.c1), x2 = load<T, V>(xs + row * a.d + at.c2);
+                    if constexpr (BACK) {
+                        y1 = load<T, V>(ys + row * a.d + at.c1);
+                        y2 = load<T, V>(ys + row * a.d + at.c2);
+                    } else {
+                        y1 = x1;
+                        y2 = x2;
+                    }
+#pragma unroll
+                    for (int i = 0; i < V / 2; ++i) {
+                        u1[i] = pair<V>(x1, i);
+                        u2[i] = pair<V>(x2, i);
+                        square = ptx::fma2(u1[i], u1[i], ptx::fma2(u2[i], u2[i], square));
+                        if constexpr (BACK) {
+                            const float2 v1 = pair<V>(y1, i), v2 = pair<V>(y2, i);
+                            g1[i] = ptx::fma2(v1, f.k1[i], ptx::mul2(v2, f.z2[i]));
+                            g2[i] = ptx::fma2(v2, f.k2[i], ptx::mul2(v1, f.z1[i]));
+                            along = ptx::fma2(ptx::mul2(g1[i], pair<V>(w.w1, i)), u1[i], ptx::fma2(ptx::mul2(g2[i], pair<V>(w.w2, i)), u2[i], along));
+                        }
+                    }
+                }
+                const float r = rsqrtf(fmaf(head_sum<LPH>(square.x + square.y), inv_d, a.eps));
+                const float back = BACK ? -head_sum<LPH>(along.x + along.y) * inv_d * r : 0.f;
+                if (!live) continue;
+                if (kind != 2) {   // (a token of no sequence passes unchanged, and so does its gradient)
+#pragma unroll
+                    for (int i = 0; i < V / 2; ++i) {
+                        if constexpr (BACK) {
+                            const float2 n1 = ptx::mul2(u1[i], both(r)), n2 = ptx::mul2(u2[i], both(r));
+                            put<V>(y1, i, ptx::mul2(ptx::fma2(n1, both(back), ptx::mul2(g1[i], pair<V>(w.w1, i))), both(r)));
+                            put<V>(y2, i, ptx::mul2(ptx::fma2(n2, both(back), ptx::mul2(g2[i], pair<V>(w.w2, i))), both(r)));
+                            d1[i] = ptx::fma2(g1[i], n1, d1[i]);
+                            d2[i] = ptx::fma2(g2[i], n2, d2[i]);
+                        } else {
+                            put<V>(y1, i, ptx::mul2(ptx::fma2(u1[i], f.k1[i], ptx::mul2(u2[i], f.z1[i])), both(r)));
+                            put<V>(y2, i, ptx::mul2(ptx::fma2(u2[i], f.k2[i], ptx::mul2(u1[i], f.z2[i])), both(r)));
+                        }
+                    }
+                }
+                store<T, V>(out + row * a.d + at.c1, y1);
+                store<T, V>(out + row * a.d + at.c2, y2);
+            }
+            s ^= 1;
+        }
+        __syncwarp();
+    }
+    if (failed) {
+        // A copy did not come: the call has failed and says so; what else is on its way is waited for (again not for ever).
+        for (int s = 0; s < STAGES; ++s)
+            if (pending >> s & 1u) ptx::mbar_wait(bars + 8 * s, phase >> s & 1u);
+        if (lane == 0) atomicOr(&g_qk_norm_status, 16u);
+    }
+    if constexpr (BACK) {
+        __syncthreads();   // (the sums lie over the rings)
+        leave_part<V, LPH, NW>(a, at, d1, d2, reinterpret_cast<float *>(smem + 128));
+    }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -327,13 +543,14 @@ __global__ void __launch_bounds__(THREADS) qk_norm_elements_kernel(NormArgs a, i
     float d1[EACH], d2[EACH];
 #pragma unroll
     for (int e = 0; e < EACH; ++e) d1[e] = d2[e] = 0.f;
+    Sequence seq;
     for (int64_t item = first; item < all; item += step) {
         const int64_t n = item / t.heads;
         const int h = (int)(item - n * t.heads);
         int64_t bi, ti;
         token_of(a, n, bi, ti);
         const int64_t xo = bi * t.sb + ti * t.st + h * t.sh, go = bi * t.gb + ti * t.gt + h * t.gh, oo = item * a.d;
-        const int64_t row = table_row(a, n, ti);
+        const int64_t row = table_row(a, n, ti, seq);
         float u1[EACH], u2[EACH], g1[EACH], g2[EACH], square = 0.f, along = 0.f;
 #pragma unroll
         for (int e = 0; e < EACH; ++e) {
@@ -442,60 +659,103 @@ __global__ void __launch_bounds__(THREADS) qk_norm_sum_kernel(NormArgs a, int bl
 // ---------------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------------
+enum Way { ELEMENTS, HEADS, RING };
 struct Plan {
-    bool vec;
+    Way way;
     int lph;                 // lanes of a head
-    int units_q, units_k;    // warps of a token
-    int blocks_q, blocks;    // backward, and the element kernels
+    int units_q, units_k;    // HEADS: warps of a token
+    RingPlan ring_q, ring_k;
+    int blocks_q, blocks;    // the ring's and the element kernels' blocks: the queries', and all
 };
 
-constexpr int HEADS_EACH = 2;   // heads of a lane
-constexpr int MAX_BLOCKS = 148 * 8;
+constexpr int HEADS_EACH = 2;          // loads of a token's heads by a warp of the kernel of few tokens
+constexpr int MAX_BLOCKS = 148 * 8;    // rows of the backward's scratch
 
 Plan plan_of(int dtype, const NormArgs &a, bool back) {
     const int eb = dtype == 0 ? 4 : 2, v = 16 / eb;
     auto aligned = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-    auto ok = [&](const NormTensor &t) {
+    auto vectors = [&](const NormTensor &t) {
         return t.heads == 0 || (aligned(t.x) && aligned(t.out) && t.sb % v == 0 && t.st % v == 0 && t.sh % v == 0 && aligned(t.w) &&
                                 (!back || (aligned(t.g) && t.gb % v == 0 && t.gt % v == 0 && t.gh % v == 0)));
     };
     Plan p{};
-    p.vec = a.dim % (2 * v) == 0 && a.d % (2 * v) == 0 && aligned(a.cos) && aligned(a.sin) && ok(a.q) && ok(a.k);
+    const bool vec = a.dim % (2 * v) == 0 && a.d % (2 * v) == 0 && aligned(a.cos) && aligned(a.sin) && vectors(a.q) && vectors(a.k);
     const int items = a.d / (2 * v);
     p.lph = items <= 4 ? 4 : items <= 8 ? 8 : items <= 16 ? 16 : 32;
-    const int per = 32 / p.lph * HEADS_EACH;
-    p.units_q = (a.q.heads + per - 1) / per;
-    p.units_k = (a.k.heads + per - 1) / per;
-    // Blocks that run until the tokens are done: eight a multiprocessor, the keys' share of them by their units.
-    const int64_t tokens = a.b * a.t, uq = p.vec ? p.units_q : a.q.heads, uk = p.vec ? p.units_k : a.k.heads;
-    const int64_t want_q = (tokens * uq + WARPS - 1) / WARPS, want_k = (tokens * uk + WARPS - 1) / WARPS, room = MAX_BLOCKS;
+    const int ng = 32 / p.lph;
+    const int64_t tokens = a.b * a.t;
+    const int hg = back ? Ring<true>::HG : Ring<false>::HG, nw = back ? Ring<true>::WARPS : Ring<false>::WARPS;
+    const int room = 148 * (back ? Ring<true>::BLOCKS : Ring<false>::BLOCKS);
+    // Warps that the tensors have work for, and what it costs, in loads of `ng` heads: a stage costs about as much as one and a half for its
+    // waiting and its factors, and where it is of several tokens their factors with every load (16384 tokens of 32 / 8 heads of 128, these
+    // counted like the others | as here: 71.6 | 63.7 us, backward 108 | 98: the blocks of one tensor waited for the other's).
+    int64_t want_q, want_k;
+    double cost_q, cost_k;
+    auto ring = [&](RingPlan &r, const NormTensor &t, int64_t &want, double &cost) {
+        // As many heads as a stage holds; where a token has at most half as many, several tokens.
+        r.heads = std::min(t.heads, ng * hg);
+        while (r.heads > ng && stage_bytes(back, r.heads, 1, a.d, a.dim, eb) > STAGE_MOST) r.heads -= ng;
+        r.units = r.heads ? (t.heads + r.heads - 1) / r.heads : 0;
+        r.tokens = r.heads ? std::max(1, std::min(32, ng * hg / r.heads)) : 1;
+        if (tokens < (int64_t)r.tokens * room * nw / 2) r.tokens = 1;   // (few tokens: rather more warps)
+        while (r.tokens > 1 && stage_bytes(back, r.heads * r.tokens, r.tokens, a.d, a.dim, eb) > STAGE_MOST) --r.tokens;
+        r.stage = stage_bytes(back, r.heads * r.tokens, r.tokens, a.d, a.dim, eb);
+        if (r.heads) r.over_heads = over_of(r.heads);
+        want = ((tokens + r.tokens - 1) / r.tokens * r.units + nw - 1) / nw;
+        cost = r.units * ((double)((r.heads * r.tokens + ng - 1) / ng) * (r.tokens == 1 ? 1.0 : back ? 1.4 : 2.2) + 1.5) / r.tokens;
+    };
+    ring(p.ring_q, a.q, want_q, cost_q);
+    ring(p.ring_k, a.k, want_k, cost_k);
+    // The ring for the gradient, and forward in 16 bits where its warps get two stages each or more: one stage alone is waited for (us, ring |
+    // a warp for every token: bf16, 32 / 8 heads of 128, 4096 tokens 18.4 | 23.4, 16384 64 | 92, 1024 6.8 | 6.8; 16 / 4 of 64, 4096 11.9 | 8.6,
+    // 16384 24 | 33).  In f32 a byte has half the instructions, and loads into registers keep up with HBM: 8192 tokens 69 | 58.
+    p.way = !vec ? ELEMENTS : back || (eb == 2 && want_q + want_k >= 2 * room) ? RING : HEADS;
+    if (p.way == HEADS) {
+        p.units_q = (a.q.heads + ng * HEADS_EACH - 1) / (ng * HEADS_EACH);
+        p.units_k = (a.k.heads + ng * HEADS_EACH - 1) / (ng * HEADS_EACH);
+        return p;
+    }
+    const int most = p.way == RING ? room : MAX_BLOCKS;
+    if (p.way == ELEMENTS) {
+        want_q = (tokens * a.q.heads + WARPS - 1) / WARPS;
+        want_k = (tokens * a.k.heads + WARPS - 1) / WARPS;
+        cost_q = a.q.heads;
+        cost_k = a.k.heads;
+    }
     int64_t bq = want_q, bk = want_k;
-    if (bq + bk > room) {
-        bk = want_k == 0 ? 0 : std::max<int64_t>(1, room * uk / (uq + uk));
-        bq = want_q == 0 ? 0 : room - bk;
+    if (bq + bk > most) {   // blocks that run until the tokens are done, the keys' share of them by what they cost
+        bk = want_k == 0 ? 0 : want_q == 0 ? most : std::min<int64_t>(most - 1, std::max<int64_t>(1, (int64_t)(most * cost_k / (cost_q + cost_k) + 0.5)));
+        bq = most - bk;
     }
     p.blocks_q = (int)bq;
     p.blocks = (int)(bq + bk);
     return p;
 }
 
+template <typename T, typename TW, int V, int LPH, bool BACK>
+cudaError_t run_ring(const NormArgs &a, const Plan &p, cudaStream_t stream) {
+    using R = Ring<BACK>;
+    const auto kernel = qk_norm_ring_kernel<T, TW, V, LPH, BACK>;
+    const int bytes = 128 + std::max(R::WARPS * R::STAGES * std::max(p.ring_q.stage, p.ring_k.stage), BACK ? R::WARPS * a.d * 4 : 0);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 + R::WARPS * R::STAGES * STAGE_MOST);
+    if (e != cudaSuccess) return e;
+    kernel<<<p.blocks, R::WARPS * 32, bytes, stream>>>(a, p.ring_q, p.ring_k, p.blocks_q);
+    return cudaGetLastError();
+}
+
 template <typename T, typename TW, int V, int LPH>
 cudaError_t run_vec(const NormArgs &a, const Plan &p, bool back, cudaStream_t stream) {
-    if (back) {
-        qk_norm_backward_kernel<T, TW, V, LPH, HEADS_EACH>
-            <<<p.blocks, THREADS, sizeof(float) * WARPS * a.d, stream>>>(a, p.units_q, p.units_k, p.blocks_q);
-    } else {
-        const int64_t blocks = (a.b * a.t * (p.units_q + p.units_k) + WARPS - 1) / WARPS;
-        if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-        qk_norm_kernel<T, TW, V, LPH, HEADS_EACH><<<(unsigned)blocks, THREADS, 0, stream>>>(a, p.units_q, p.units_k);
-    }
+    if (p.way == RING) return back ? run_ring<T, TW, V, LPH, true>(a, p, stream) : run_ring<T, TW, V, LPH, false>(a, p, stream);
+    const int64_t blocks = (a.b * a.t * (p.units_q + p.units_k) + WARPS - 1) / WARPS;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+    qk_norm_kernel<T, TW, V, LPH, HEADS_EACH><<<(unsigned)blocks, THREADS, 0, stream>>>(a, p.units_q, p.units_q + p.units_k, over_of(p.units_q + p.units_k));
     return cudaGetLastError();
 }
 
 template <typename T, typename TW>
 cudaError_t run_t(const NormArgs &a, const Plan &p, bool back, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
-    if (!p.vec) {
+    if (p.way == ELEMENTS) {
         if (back) qk_norm_elements_kernel<T, true><<<p.blocks, THREADS, sizeof(float) * WARPS * a.d, stream>>>(a, p.blocks_q);
         else qk_norm_elements_kernel<T, false><<<p.blocks, THREADS, 0, stream>>>(a, p.blocks_q);
         return cudaGetLastError();
@@ -518,19 +778,32 @@ cudaError_t run(int dtype, const NormArgs &a, const Plan &p, bool back, cudaStre
 
 bool nothing(const NormArgs &a) { return a.b * a.t == 0 || a.q.heads + a.k.heads == 0 || a.d == 0; }
 
+// Where a token's position does not go by its batch element, and every tensor's batch elements follow one another, they are one.
+NormArgs prepared(NormArgs a) {
+    auto one = [&](const NormTensor &t) { return t.heads == 0 || (t.sb == a.t * t.st && (!t.g || t.gb == a.t * t.gt)); };
+    if (a.b > 1 && (a.positions || a.cu) && one(a.q) && one(a.k)) {
+        a.t *= a.b;
+        a.b = 1;
+    }
+    if (a.t < (int64_t(1) << 31)) a.over_t = over_of(a.t);
+    return a;
+}
+
 }  // namespace
 
 // As many rows as the larger of the two ways needs: which one runs depends on addresses, which a workspace query does not have.
 size_t qk_norm_part_floats(int d) { return (size_t)MAX_BLOCKS * d; }
 
-cudaError_t launch_qk_norm(int dtype, const NormArgs &a, cudaStream_t stream, int *launches) {
-    if (nothing(a)) return cudaSuccess;
+cudaError_t launch_qk_norm(int dtype, const NormArgs &given, cudaStream_t stream, int *launches) {
+    if (nothing(given)) return cudaSuccess;
+    const NormArgs a = prepared(given);
     *launches += 1;
     return run(dtype, a, plan_of(dtype, a, false), false, stream);
 }
 
-cudaError_t launch_qk_norm_backward(int dtype, const NormArgs &a, cudaStream_t stream, int *launches) {
-    if (nothing(a)) return cudaSuccess;
+cudaError_t launch_qk_norm_backward(int dtype, const NormArgs &given, cudaStream_t stream, int *launches) {
+    if (nothing(given)) return cudaSuccess;
+    const NormArgs a = prepared(given);
     const Plan p = plan_of(dtype, a, true);
     *launches += 1;
     cudaError_t e = run(dtype, a, p, true, stream);
@@ -540,6 +813,16 @@ cudaError_t launch_qk_norm_backward(int dtype, const NormArgs &a, cudaStream_t s
     if (dtype == 0 || a.w_f32) return launch_beside(qk_norm_sum_kernel<float>, grid, THREADS, 0, stream, true, a, p.blocks_q, p.blocks);
     if (dtype == 1) return launch_beside(qk_norm_sum_kernel<__nv_bfloat16>, grid, THREADS, 0, stream, true, a, p.blocks_q, p.blocks);
     return launch_beside(qk_norm_sum_kernel<__half>, grid, THREADS, 0, stream, true, a, p.blocks_q, p.blocks);
+}
+
+cudaError_t read_qk_norm_status(unsigned int *status, bool clear) {
+    cudaError_t e = cudaMemcpyFromSymbol(status, g_qk_norm_status, sizeof(unsigned int));
+    if (e != cudaSuccess) return e;
+    if (clear && *status) {
+        unsigned int zero = 0;
+        e = cudaMemcpyToSymbol(g_qk_norm_status, &zero, sizeof(unsigned int));
+    }
+    return e;
 }
 
 }  // namespace dash

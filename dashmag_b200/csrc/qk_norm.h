@@ -18,6 +18,8 @@ struct NormTensor {
     int heads;
 };
 
+struct Over { uint32_t mul; int shift; };   // a division by a known number, as a multiplication
+
 struct NormArgs {
     NormTensor q, k;       // k.heads == 0: one tensor only.  Both share the tokens' positions.
     int b;
@@ -33,6 +35,7 @@ struct NormArgs {
     const void *cu;        // [sequences + 1] i32 / i64: start + n - cu[s] for cu[s] <= n < cu[s + 1]
     int cu_bytes, sequences;
     int64_t start;         // start + n % t
+    Over over_t;           // set by the launchers
     float *part;           // backward scratch: a row of d sums per block
 };
 
@@ -40,5 +43,8 @@ struct NormArgs {
 size_t qk_norm_part_floats(int d);
 cudaError_t launch_qk_norm(int dtype, const NormArgs &a, cudaStream_t stream, int *launches);
 cudaError_t launch_qk_norm_backward(int dtype, const NormArgs &a, cudaStream_t stream, int *launches);
+
+// The sticky device word that a bounded wait of these kernels raises when it runs out.
+cudaError_t read_qk_norm_status(unsigned int *status, bool clear);
 
 }  // namespace dash
