@@ -6,15 +6,16 @@
 //
 // in f32 and rounded once to the logits' dtype.
 //
-// A block takes a piece of one row's vocabulary and keeps a word per token of it in shared memory: the count, and the top bit for a
-// token of the prompt.  It reads the row's history, counts the ids that fall into its piece (integer additions, whose order does not
-// matter), and then makes the pass over its logits, which were asked for before the history.  Nothing is sorted and no
-// scratch is needed.  What a block waits for is one trip to memory: its logits, the grammar's words, the row's numbers and the first ids are
-// all asked for before any is looked at, the ids before it is known how many are the row's.  (One after another, four trips: 251 rows of
-// 38531 tokens with a grammar and next to no history 19.8 us, now XX.)  The pieces cost the history read once for each, from L2;
-// clusters of eight blocks that read a share each and count for one another in distributed shared memory were slower (256 rows of
-// 100003, 8192 ids, 107 us against 68: half of a text's ids are a few tokens, whose words all eight blocks then wait for).
-// The pass itself is a read and a write of the logits, bound by HBM.
+// A block takes a piece of one row's vocabulary and keeps a counter per token of it in shared memory: the count, and the top bit for a
+// token of the prompt.  It reads the row's whole history, counts the ids that fall into its piece (integer additions, whose order does not
+// matter), and then makes the pass over its logits, a chunk of a vector a thread at a time.  Nothing is sorted and no scratch is needed.
+// The first chunks, the grammar's words, the row's numbers and the first ids are all asked for before any is looked at, the ids before it is
+// known how many are the row's: a block waits for one trip to memory before it counts, and in the pass its chunks are DEPTH ahead.
+// The history is read once per piece, from L2, so pieces are long - counters of 16 bits where no history overflows them - as far as the
+// blocks still fill the GPU evenly (chunks_of).  The pass is a read and a write of the logits, bound by HBM.
+// (Pieces of 8192 tokens held in registers, counters of 32 bits, four trips one after another: 256 rows of 100003 tokens with up to 8192
+// ids 85 us, one trip 58, now 38; clusters of eight blocks that read a share of the history each and count for one another in
+// distributed shared memory 107: half of a text's ids are a few tokens, whose words all eight then wait for.)
 #include <algorithm>
 #include <type_traits>
 
@@ -24,30 +25,32 @@
 namespace dash {
 namespace {
 
-constexpr int THREADS = 256;
-#ifndef MINB
-#define MINB 3
-#define MAXE 4
-#endif
-constexpr unsigned IN_PROMPT = 0x80000000u;
+constexpr int THREADS = 512, DEPTH = 2;
+
+// Counters of tokens: bits, the mark of a prompt's token, the count.
+template <typename C> struct Counter {
+    static constexpr unsigned MARK = 1u << (8 * sizeof(C) - 1);
+    static constexpr int PER = 4 / sizeof(C);   // of a 32-bit word
+    // Adds `x` to (or sets it in) the counter at place `at`.
+    static __device__ __forceinline__ void add(unsigned *words, unsigned at) { atomicAdd(&words[at / PER], 1u << (at % PER * 8 * sizeof(C))); }
+    static __device__ __forceinline__ void mark(unsigned *words, unsigned at) { atomicOr(&words[at / PER], MARK << (at % PER * 8 * sizeof(C))); }
+    static __device__ __forceinline__ unsigned get(const unsigned *w, int e) { return w[e / PER] >> (e % PER * 8 * sizeof(C)) & (MARK | (MARK - 1)); }
+};
 
 template <typename T, int V> struct alignas(16) Vec { T e[V]; };
 
 // What a row's tokens go through.
 struct Rules {
-    float repetition, frequency, presence;
-    const uint32_t *allowed;
+    float repetition, inverse, frequency, presence;   // (inverse: of the repetition penalty)
 };
-
-// One token's logit: `word` its count and mark, `bias` and `open` the grammar's bit where there are any.
-__device__ __forceinline__ float ruled(const Rules &r, float z, unsigned word, float bias, bool open) {
-    if (word) {
-        z = z > 0.f ? z / r.repetition : z * r.repetition;
-        const unsigned count = word & ~IN_PROMPT;
-        if (count) z = z - r.frequency * (float)count - r.presence;
-    }
-    z += bias;
-    return open ? z : -INFINITY;
+// One token's logit by its counter.  (The quotient as a product with the reciprocal, a unit in the last place of f32 from it.)
+template <typename C> __device__ __forceinline__ float ruled(const Rules &r, float z, unsigned word) {
+    const float factor = z > 0.f ? r.inverse : r.repetition;
+    z *= word ? factor : 1.f;
+    const unsigned count = word & (Counter<C>::MARK - 1);
+    // (As a f32: of fewer than 24 bits by the number 2^23 they are the last bits of, off the conversions' pipe.)
+    const float times = sizeof(C) == 2 ? __uint_as_float(0x4b000000u | count) - 8388608.f : (float)count;
+    return fmaf(-r.frequency, times, z) - (count ? r.presence : 0.f);
 }
 
 // Index i of an array of i32 / i64 as it stands there; `none` where there is no array.
@@ -56,21 +59,23 @@ __device__ __forceinline__ int64_t number(const void *p, int bytes, int i, int n
 }
 __device__ __forceinline__ int within(int64_t x, int top) { return (int)min(max(x, (int64_t)0), (int64_t)top); }
 
-constexpr int AHEAD = 8;   // ids of a thread on their way at once
+constexpr int AHEAD = 4;   // ids of a thread on their way at once
 
-// EACH vectors a thread: a piece of THREADS * EACH * V tokens.  I: the ids' integers.
-template <typename T, typename I, int EACH>
-__global__ void __launch_bounds__(THREADS, MINB) penalize_kernel(PenalizeArgs a, int pieces) {
-    constexpr int V = 16 / sizeof(T), PIECE = THREADS * EACH * V;
-    __shared__ alignas(16) unsigned words[PIECE];
+// A block a piece of `chunks` times THREADS * V places.  I: the ids' integers, C: the counters'.
+template <typename T, typename I, typename C>
+__global__ void __launch_bounds__(THREADS, 2) penalize_kernel(PenalizeArgs a, int pieces, int chunks) {
+    constexpr int V = 16 / sizeof(T), CHUNK = THREADS * V, WORDS = V * sizeof(C) / 4;
+    extern __shared__ uint4 smem[];
+    unsigned *words = reinterpret_cast<unsigned *>(smem);
     const int row = blockIdx.x / pieces, piece = blockIdx.x - row * pieces;
     const T *in = static_cast<const T *>(a.logits) + (int64_t)row * a.stride;
     T *out = static_cast<T *>(a.out) + (int64_t)row * a.out_stride;
     // Places are counted from the 16-byte boundary at or before the row, so that whole vectors are aligned whatever the row's address.
     const int skew = (int)((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));
     const bool vec = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-    const int first = piece * PIECE - skew;   // the token of the piece's first place (negative: there is none)
+    const int places = chunks * CHUNK, first = piece * places - skew;   // the token of the piece's first place (negative: there is none)
     if (first >= a.v) return;
+    const int last = (int)min((int64_t)first + places, (int64_t)a.v);   // past the piece's last token
 
     const I *ids = static_cast<const I *>(a.ids) + (int64_t)row * a.ids_stride;
     I id[AHEAD];
@@ -86,30 +91,27 @@ __global__ void __launch_bounds__(THREADS, MINB) penalize_kernel(PenalizeArgs a,
     }
     Rules r;
     r.repetition = a.repetition ? a.repetition[row] : a.repetition_all;
+    r.inverse = 1.f / r.repetition;
     r.frequency = a.frequency ? a.frequency[row] : a.frequency_all;
     r.presence = a.presence ? a.presence[row] : a.presence_all;
-    r.allowed = a.allowed ? a.allowed + (int64_t)row * a.allowed_stride : nullptr;
-    Vec<T, V> x[EACH];
-    uint32_t open[EACH], open2[EACH];   // the words a whole vector's V bits lie in
-    auto token = [&](int j) { return first + (j * THREADS + (int)threadIdx.x) * V; };
+    const uint32_t *allowed = a.allowed ? a.allowed + (int64_t)row * a.allowed_stride : nullptr;
+    Vec<T, V> x[DEPTH];
+    uint32_t open[DEPTH], open2[DEPTH];   // the words that hold a whole vector's bits of the grammar: one, or two where the row begins off a boundary
     auto whole = [&](int v0) { return vec && v0 >= 0 && v0 <= a.v - V; };
-#pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-        const int v0 = token(j);
-        if (whole(v0)) {
-            *reinterpret_cast<uint4 *>(&x[j]) = *reinterpret_cast<const uint4 *>(in + v0);
-            if (r.allowed) {
-                open[j] = r.allowed[v0 >> 5];
-                open2[j] = skew ? r.allowed[(v0 + V - 1) >> 5] : 0;
+    auto fetch = [&](int v0, Vec<T, V> &x, uint32_t &open, uint32_t &open2) {
+        if (v0 < last && whole(v0)) {
+            *reinterpret_cast<uint4 *>(&x) = *reinterpret_cast<const uint4 *>(in + v0);
+            if (allowed) {   // (not looked at before the pass: that would be a wait for them here)
+                open = allowed[v0 >> 5];
+                if (skew) open2 = allowed[(v0 + V - 1) >> 5];
             }
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (v0 + e >= 0 && v0 + e < a.v) x[j].e[e] = in[v0 + e];
         }
-    }
+    };
+    const int v_first = first + (int)threadIdx.x * V;
+#pragma unroll
+    for (int j = 0; j < DEPTH; ++j) fetch(v_first + j * CHUNK, x[j], open[j], open2[j]);
     if (a.ids) {
-        for (int i = threadIdx.x; i < PIECE / 4; i += THREADS) reinterpret_cast<uint4 *>(words)[i] = make_uint4(0, 0, 0, 0);
+        for (int i = threadIdx.x; i < places / (4 * Counter<C>::PER); i += THREADS) smem[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
         const int len = within(length, a.t), prompt = within(prompt_length, len);
         for (int i0 = threadIdx.x; i0 < len; i0 += THREADS * AHEAD) {
@@ -119,9 +121,9 @@ __global__ void __launch_bounds__(THREADS, MINB) penalize_kernel(PenalizeArgs a,
                 // (Ids outside the vocabulary, padding's -1 among them, count for nothing; another piece's come out past this one's places.)
                 const unsigned at = (unsigned)((int)id[e] - first);
                 const int i = i0 + e * THREADS;
-                if ((std::make_unsigned_t<I>)id[e] >= (std::make_unsigned_t<I>)a.v || at >= (unsigned)PIECE || i >= len) continue;
-                if (i < prompt) atomicOr(&words[at], IN_PROMPT);
-                else atomicAdd(&words[at], 1u);
+                if ((std::make_unsigned_t<I>)id[e] >= (std::make_unsigned_t<I>)a.v || at >= (unsigned)places || i >= len) continue;
+                if (i < prompt) Counter<C>::mark(words, at);
+                else Counter<C>::add(words, at);
             }
         }
         __syncthreads();
@@ -131,34 +133,42 @@ __global__ void __launch_bounds__(THREADS, MINB) penalize_kernel(PenalizeArgs a,
     auto bias_at = [&](int v) {
         return a.bias_f32 ? static_cast<const float *>(a.bias)[bias0 + v] : Num<T>::to_f32(static_cast<const T *>(a.bias)[bias0 + v]);
     };
-#pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-        const int v0 = token(j);
-        if (v0 >= a.v || v0 + V <= 0) continue;
-        unsigned w[V], any = 0;
-#pragma unroll
-        for (int e = 0; e < V; ++e) w[e] = 0;
+    auto pass = [&](int v0, const Vec<T, V> &x, uint32_t bits) {
+        alignas(16) unsigned w[WORDS];
         if (a.ids) {
+            const unsigned *at = words + (v0 - first) / Counter<C>::PER;
 #pragma unroll
-            for (int e = 0; e < V; e += 4) *reinterpret_cast<uint4 *>(&w[e]) = reinterpret_cast<const uint4 *>(words)[((j * THREADS + threadIdx.x) * V + e) / 4];
-#pragma unroll
-            for (int e = 0; e < V; ++e) any |= w[e];
+            for (int e = 0; e < WORDS; e += WORDS < 4 ? 2 : 4) {
+                if constexpr (WORDS < 4) *reinterpret_cast<uint2 *>(&w[e]) = *reinterpret_cast<const uint2 *>(at + e);
+                else *reinterpret_cast<uint4 *>(&w[e]) = *reinterpret_cast<const uint4 *>(at + e);
+            }
         }
         if (!whole(v0)) {   // the row's ends
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const int v = v0 + e;
-                if (v >= 0 && v < a.v)
-                    out[v] = Num<T>::from_f32(ruled(r, Num<T>::to_f32(x[j].e[e]), w[e], a.bias ? bias_at(v) : 0.f, !r.allowed || (r.allowed[v >> 5] >> (v & 31) & 1u)));
+                if (v < 0 || v >= a.v) continue;
+                float z = Num<T>::to_f32(in[v]);
+                if (a.ids) z = ruled<C>(r, z, Counter<C>::get(w, e));
+                if (a.bias) z += bias_at(v);
+                if (allowed && !(allowed[v >> 5] >> (v & 31) & 1u)) z = -INFINITY;
+                out[v] = Num<T>::from_f32(z);
             }
-            continue;
+            return;
         }
         float z[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) z[e] = Num<T>::to_f32(x[j].e[e]);
-        if (any) {
+        for (int e = 0; e < V; ++e) z[e] = Num<T>::to_f32(x.e[e]);
+        if (a.ids) {
+            // (All of a vector or nothing: a history of some thousands touches one vector in ten, nearly every warp's 32 of them.  Word by
+            // word the branches cost more than they spare, 256 rows of 100003 with up to 8192 ids 38.1 us against 42.8.)
+            unsigned any = 0;
 #pragma unroll
-            for (int e = 0; e < V; ++e) z[e] = ruled(r, z[e], w[e], 0.f, true);
+            for (int i = 0; i < WORDS; ++i) any |= w[i];
+            if (any) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) z[e] = ruled<C>(r, z[e], Counter<C>::get(w, e));
+            }
         }
         if (a.bias) {
             const bool four = a.bias_f32 && (reinterpret_cast<uintptr_t>(static_cast<const float *>(a.bias) + bias0 + v0) & 15) == 0;
@@ -173,8 +183,7 @@ __global__ void __launch_bounds__(THREADS, MINB) penalize_kernel(PenalizeArgs a,
                 for (int e = 0; e < V; ++e) z[e] += bias_at(v0 + e);
             }
         }
-        if (r.allowed) {
-            const uint32_t bits = __funnelshift_r(open[j], open2[j], v0 & 31);
+        if (allowed) {
 #pragma unroll
             for (int e = 0; e < V; ++e) z[e] = bits >> e & 1u ? z[e] : -INFINITY;
         }
@@ -182,26 +191,56 @@ __global__ void __launch_bounds__(THREADS, MINB) penalize_kernel(PenalizeArgs a,
 #pragma unroll
         for (int e = 0; e < V; ++e) y.e[e] = Num<T>::from_f32(z[e]);
         *reinterpret_cast<uint4 *>(out + v0) = *reinterpret_cast<const uint4 *>(&y);
+    };
+    for (int v0 = v_first; v0 < last; v0 += DEPTH * CHUNK) {
+#pragma unroll
+        for (int j = 0; j < DEPTH; ++j) {
+            const int v = v0 + j * CHUNK;
+            if (v >= last) break;
+            const Vec<T, V> now = x[j];
+            const uint32_t bits = open[j], bits2 = open2[j];
+            fetch(v + DEPTH * CHUNK, x[j], open[j], open2[j]);
+            pass(v, now, skew ? __funnelshift_r(bits, bits2, v & 31) : bits >> (v & 31));
+        }
     }
 }
 
-template <typename T, int EACH>
-cudaError_t run(const PenalizeArgs &a, int pieces, cudaStream_t stream) {
-    const int64_t blocks = (int64_t)pieces * a.b;
+constexpr int MOST_BYTES = 96 * 1024;   // of counters: two blocks a multiprocessor
+
+// Chunks of a piece.  The blocks run in waves of two a multiprocessor; a block costs its chunks, and about three and a half of them until
+// its first is there, and the history.
+int chunks_of(int64_t chunks_of_row, int b, int t, int most) {
+    int best = 1;
+    double least = 0.;
+    for (int k = 1; k <= most; ++k) {
+        const int64_t blocks = (chunks_of_row + k - 1) / k * b, waves = (blocks + 2 * 148 - 1) / (2 * 148);
+        const double cost = waves * (k + 3.5 + t / 3000.);
+        if (k == 1 || cost < least) { best = k; least = cost; }
+        if (k >= chunks_of_row) break;
+    }
+    return best;
+}
+
+template <typename T, typename I, typename C>
+cudaError_t run(const PenalizeArgs &a, cudaStream_t stream) {
+    constexpr int CHUNK = THREADS * 16 / (int)sizeof(T);
+    const int64_t row = ((int64_t)a.v + 16 / (int)sizeof(T) - 1 + CHUNK - 1) / CHUNK;
+    const int chunks = chunks_of(row, a.b, a.ids ? a.t : 0, MOST_BYTES / (CHUNK * (int)sizeof(C)));
+    const int64_t pieces = (row + chunks - 1) / chunks, blocks = pieces * a.b;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-    if (a.ids_bytes == 8) penalize_kernel<T, int64_t, EACH><<<(unsigned)blocks, THREADS, 0, stream>>>(a, pieces);
-    else penalize_kernel<T, int32_t, EACH><<<(unsigned)blocks, THREADS, 0, stream>>>(a, pieces);
+    const auto kernel = penalize_kernel<T, I, C>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_BYTES);
+    if (e != cudaSuccess) return e;
+    kernel<<<(unsigned)blocks, THREADS, a.ids ? (size_t)chunks * CHUNK * sizeof(C) : 0, stream>>>(a, (int)pieces, chunks);
     return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t penalize_t(const PenalizeArgs &a, cudaStream_t stream) {
-    constexpr int V = 16 / sizeof(T);
-    auto pieces = [&](int each) { return (int)(((int64_t)a.v + V - 1 + THREADS * each * V - 1) / (THREADS * each * V)); };
-    // The largest piece (the history is read once per piece) that still leaves four blocks to a multiprocessor.
-    int each = MAXE;
-    while (each > 1 && (int64_t)pieces(each) * a.b < 148 * 4) each /= 2;
-    return each == 4 ? run<T, 4>(a, pieces(4), stream) : each == 2 ? run<T, 2>(a, pieces(2), stream) : run<T, 1>(a, pieces(1), stream);
+    // (A counter of 16 bits counts to 32767.)
+    const bool small = !a.ids || a.t <= 0x7fff;
+    if (a.ids_bytes == 8) return small ? run<T, int64_t, uint16_t>(a, stream) : run<T, int64_t, uint32_t>(a, stream);
+    return small ? run<T, int32_t, uint16_t>(a, stream) : run<T, int32_t, uint32_t>(a, stream);
 }
 
 }  // namespace
