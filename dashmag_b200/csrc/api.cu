@@ -732,7 +732,10 @@ struct PrefixSpace {
 static PrefixSpace prefix_space(const dash_attn_decode_params *p, const dash_attn_prefix_params *x) {
     PrefixSpace s{};
     const int each = p->b / x->n;
-    s.tensor = dash::sm100_prefix_splits(p->dtype, scale_for(p->has_scale, p->scale, p->d), x->n, each, x->p, p->hq, p->hkv, p->d);
+    // What the own keys may come to: under a window it, and of caches with lengths about half.
+    const double seen = p->has_window && p->window_left >= 0 ? (double)std::min<int64_t>(p->window_left + (p->window_left < p->s), p->s) : p->lengths ? 0.55 * p->s : p->s;
+    const double own_bytes = seen * p->b * p->hkv * p->d * 2. * (double)elem_bytes(p->dtype);
+    s.tensor = dash::sm100_prefix_splits(p->dtype, scale_for(p->has_scale, p->scale, p->d), x->n, each, x->p, p->hq, p->hkv, p->d, own_bytes);
     s.generic = dash::prefix_generic_splits(x->n, each, x->p, p->hq, p->hkv);
     const size_t rows = (size_t)p->b * p->hq, splits = (size_t)std::max(s.tensor, s.generic);
     s.part_o = align256(sizeof(float) * rows * splits * p->d);
@@ -803,22 +806,17 @@ int dash_attn_decode_shared(const dash_attn_decode_params *p, const dash_attn_pr
 
     int launches = 0;
     cudaError_t e = cudaSuccess;
-    const bool both = p->s > 0;
-    if (both) e = dash::launch_decode_parts(p->dtype, own, decode_vectors(p, q, k_new, v_new, k_cache, v_cache), stream, &launches);
-    if (e == cudaSuccess) {
-        if (s.tensor > 0 && !g_force_generic.load() && dash::sm100_prefix_takes(a)) {
-            a.splits = s.tensor;
-            if (!dash::sm100_prefix(p->dtype, a, both, stream, &launches, &e)) {
-                g_probe[DASH_ATTN_PROBE_KERNEL_LAUNCHES] += launches;
-                return fail(DASH_ATTN_CUDA, "%s: the driver refused a TMA tensor map over the inputs", op);
-            }
-            g_probe[DASH_ATTN_PROBE_TENSOR_CORE_RUNS] += 1;
-        } else {
-            a.splits = s.generic;
-            e = dash::launch_prefix_generic(p->dtype, a, both, stream, &launches);
-            g_probe[DASH_ATTN_PROBE_GENERIC_RUNS] += 1;
-        }
+    if (s.tensor > 0 && !g_force_generic.load() && dash::sm100_prefix_takes(a)) {
+        a.splits = s.tensor;
+        if (!dash::sm100_prefix(p->dtype, a, stream, &launches, &e)) return fail(DASH_ATTN_CUDA, "%s: the driver refused a TMA tensor map over the inputs", op);
+        g_probe[DASH_ATTN_PROBE_TENSOR_CORE_RUNS] += 1;
+    } else {
+        a.splits = s.generic;
+        e = dash::launch_prefix_generic(p->dtype, a, stream, &launches);
+        g_probe[DASH_ATTN_PROBE_GENERIC_RUNS] += 1;
     }
+    if (e == cudaSuccess && p->s > 0)
+        e = dash::launch_decode_parts(p->dtype, own, decode_vectors(p, q, k_new, v_new, k_cache, v_cache), true, stream, &launches);
     if (e == cudaSuccess) {
         const dash::PrefixMergeArgs m{(int64_t)p->b * p->hq, p->hq, p->d, a.splits, a.part_o, a.part_lse, own, out};
         e = dash::launch_prefix_merge(p->dtype, m, stream, &launches);

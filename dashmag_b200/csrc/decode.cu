@@ -146,8 +146,13 @@ __device__ __forceinline__ void slot8<__half>(const uint4 *slot, float (&x)[8]) 
 // The bytes in flight therefore cost shared memory, not registers, no lane ever waits for
 // another, and a multiprocessor keeps three blocks of four such warps resident: twelve warps
 // with three steps each on the way from HBM.
-template <typename T, int D, int GH>
+// JOIN (launch_decode_parts): beside the launch in front; a block more a sequence, the last of which waits for that launch's end.  (An instance
+// of its own, and in front of everything else: a wait at a return costs registers, and the tensor-core pass a block of a multiprocessor's two.)
+template <typename T, int D, int GH, bool JOIN>
 __global__ void __launch_bounds__(DEC_WARPS * 32) decode_split_kernel(DecodeArgs a) {
+    if constexpr (JOIN) {
+        if (blockIdx.x == gridDim.x - 1) { end_beside(); return; }
+    }
     allow_beside();   // the merge
     constexpr int LPK = D / 8;                    // lanes per key
     constexpr int KPW = 32 / LPK;                 // keys per warp in one load
@@ -422,8 +427,11 @@ __device__ __forceinline__ void cluster_store(void *mine, int rank, float2 v) {
     asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(cluster_address(mine, rank)), "f"(v.x), "f"(v.y) : "memory");
 }
 
-template <typename T, int D, int PARTS, bool WIDE, int WARPS, bool ROPE, bool CLUSTER>
+template <typename T, int D, int PARTS, bool WIDE, int WARPS, bool ROPE, bool CLUSTER, bool JOIN>
 __global__ void __launch_bounds__(WARPS * 32) decode_split_mma_kernel(DecodeArgs a) {
+    if constexpr (JOIN) {
+        if (blockIdx.x == gridDim.x - 1) { end_beside(); return; }
+    }
     constexpr int DM_WARPS = WARPS;
     if constexpr (!CLUSTER) allow_beside();   // the merge
     constexpr int DFULL = D * PARTS;            // the head dimension; D is what one warp takes of it
@@ -886,8 +894,11 @@ __global__ void __launch_bounds__(WARPS * 32) decode_split_mma_kernel(DecodeArgs
 
 // The same split for inputs the vector loads cannot take: one warp per (chunk, query head), a
 // lane owning the head dimensions `lane + 32 i`, keys in order.
-template <typename T>
+template <typename T, bool JOIN>
 __global__ void __launch_bounds__(DEC_WARPS * 32) decode_split_scalar_kernel(DecodeArgs a) {
+    if constexpr (JOIN) {
+        if (blockIdx.x == gridDim.x - 1) { end_beside(); return; }
+    }
     allow_beside();   // the merge
     const int lane = threadIdx.x & 31;
     const int b = blockIdx.y;
@@ -1097,25 +1108,25 @@ __global__ void __launch_bounds__(TH) decode_merge_kernel(DecodeArgs a) {
 }
 
 template <typename T, int D, int GH>
-static cudaError_t split_vec_g(const DecodeArgs &a, dim3 grid, cudaStream_t stream) {
+static cudaError_t split_vec_g(const DecodeArgs &a, dim3 grid, bool beside, cudaStream_t stream) {
     constexpr int VPK = sizeof(T) == 4 ? 2 : 1, NS = sizeof(T) == 4 ? 2 : DEC_STAGES;
     constexpr size_t smem = (size_t)DEC_WARPS * NS * (2 * DEC_UNROLL * VPK) * 32 * 16;
-    cudaError_t e = cudaFuncSetAttribute(decode_split_kernel<T, D, GH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const auto kernel = beside ? decode_split_kernel<T, D, GH, true> : decode_split_kernel<T, D, GH, false>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    decode_split_kernel<T, D, GH><<<grid, DEC_WARPS * 32, smem, stream>>>(a);
-    return cudaGetLastError();
+    return launch_beside(kernel, grid, DEC_WARPS * 32, smem, stream, beside, a);
 }
 
 template <typename T, int D>
-static cudaError_t split_vec(const DecodeArgs &a, cudaStream_t stream) {
+static cudaError_t split_vec(const DecodeArgs &a, bool beside, cudaStream_t stream) {
     const int group = a.hq / a.hkv;
     const int gh = group >= 4 ? 4 : (group >= 2 ? 2 : 1);
     const int passes = (group + gh - 1) / gh;
     const long long units = (long long)a.splits * a.hkv * passes;
-    dim3 grid((unsigned)((units + DEC_WARPS - 1) / DEC_WARPS), a.b);
-    if (gh == 4) return split_vec_g<T, D, 4>(a, grid, stream);
-    if (gh == 2) return split_vec_g<T, D, 2>(a, grid, stream);
-    return split_vec_g<T, D, 1>(a, grid, stream);
+    dim3 grid((unsigned)((units + DEC_WARPS - 1) / DEC_WARPS + beside), a.b);
+    if (gh == 4) return split_vec_g<T, D, 4>(a, grid, beside, stream);
+    if (gh == 2) return split_vec_g<T, D, 2>(a, grid, beside, stream);
+    return split_vec_g<T, D, 1>(a, grid, beside, stream);
 }
 
 // Bytes of shared memory of a block of the tensor-core pass; `cluster`: with the boxes its cluster meets in (a share of the
@@ -1127,14 +1138,17 @@ constexpr size_t mma_smem(int dfull, bool wide, int warps, bool cluster) {
 }
 // `warps`: of one sequence.
 template <typename T, int DFULL, bool WIDE, int WARPS, bool CLUSTER>
-static cudaError_t split_mma_w(const DecodeArgs &a, long long warps, int cluster, cudaStream_t stream) {
+static cudaError_t split_mma_w(const DecodeArgs &a, long long warps, int cluster, bool beside, cudaStream_t stream) {
     constexpr int PARTS = DFULL > 128 ? 2 : 1, D = DFULL / PARTS;
     constexpr size_t smem = mma_smem(DFULL, WIDE, WARPS, CLUSTER);
-    const auto kernel = a.rope_cos ? decode_split_mma_kernel<T, D, PARTS, WIDE, WARPS, true, CLUSTER> : decode_split_mma_kernel<T, D, PARTS, WIDE, WARPS, false, CLUSTER>;
+    const auto kernel = a.rope_cos ? decode_split_mma_kernel<T, D, PARTS, WIDE, WARPS, true, CLUSTER, false>
+                        : beside   ? decode_split_mma_kernel<T, D, PARTS, WIDE, WARPS, false, CLUSTER, !CLUSTER>   // (never in clusters)
+                                   : decode_split_mma_kernel<T, D, PARTS, WIDE, WARPS, false, CLUSTER, false>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e == cudaSuccess && cluster > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
-    return launch_clusters(kernel, dim3((unsigned)((warps + WARPS - 1) / WARPS), (unsigned)a.b), WARPS * 32, smem, stream, false, (unsigned)cluster, a);
+    return launch_clusters(kernel, dim3((unsigned)((warps + WARPS - 1) / WARPS + beside), (unsigned)a.b), WARPS * 32, smem, stream, beside,
+                           (unsigned)cluster, a);
 }
 // Blocks (of CLUSTER_WARPS warps) of the cluster that takes a key-value head of a sequence; 0: chunks, and the merge behind them.
 // A cluster saves the merge and its launch, 3 to 5 us; what it costs is the chain of a warp's tiles (0.4 us a tile at D 64, 0.6 at 128,
@@ -1189,28 +1203,28 @@ static int decode_cluster(const DecodeArgs &a, bool narrow) {
     }
     return best;
 }
-// (`merged` null: chunks, whose parts somebody else merges.)
+// (`merged` null: chunks, whose parts somebody else merges; `beside`, then: beside the launch in front.)
 template <typename T, int DFULL>
-static cudaError_t split_mma(const DecodeArgs &a, cudaStream_t stream, bool *merged) {
+static cudaError_t split_mma(const DecodeArgs &a, bool beside, cudaStream_t stream, bool *merged) {
     const int group = a.hq / a.hkv;
     const bool wide = group > 8;
     // (A cluster stores its outputs eight bytes at a time, the merge one element: it takes any address.)
     const bool whole = reinterpret_cast<uintptr_t>(a.out) % 8 == 0;
     if (const int cluster = wide || !whole || !merged ? 0 : decode_cluster(a, MmaType<T>::NARROW)) {
         const long long warps = (long long)a.hkv * cluster * CLUSTER_WARPS;
-        const cudaError_t e = split_mma_w<T, DFULL, false, CLUSTER_WARPS, true>(a, warps, cluster, stream);
+        const cudaError_t e = split_mma_w<T, DFULL, false, CLUSTER_WARPS, true>(a, warps, cluster, false, stream);
         *merged = e == cudaSuccess;
         if (*merged) return e;
         cudaGetLastError();   // (a part of a GPU may have no room for such a cluster: the chunks go anywhere)
     }
     const long long warps = (long long)a.splits * a.hkv * (wide ? (group + 15) / 16 : 1) * (DFULL > 128 ? 2 : 1);   // of one sequence
     const bool few = warps * a.b < 148LL * 8 * 2;
-    if (wide) return few ? split_mma_w<T, DFULL, true, 2, false>(a, warps, 1, stream) : split_mma_w<T, DFULL, true, 8, false>(a, warps, 1, stream);
-    return few ? split_mma_w<T, DFULL, false, 2, false>(a, warps, 1, stream) : split_mma_w<T, DFULL, false, 8, false>(a, warps, 1, stream);
+    if (wide) return few ? split_mma_w<T, DFULL, true, 2, false>(a, warps, 1, beside, stream) : split_mma_w<T, DFULL, true, 8, false>(a, warps, 1, beside, stream);
+    return few ? split_mma_w<T, DFULL, false, 2, false>(a, warps, 1, beside, stream) : split_mma_w<T, DFULL, false, 8, false>(a, warps, 1, beside, stream);
 }
-template <> cudaError_t split_mma<float, 128>(const DecodeArgs &, cudaStream_t, bool *) { return cudaErrorInvalidValue; }   // never taken: 16-bit caches only
-template <> cudaError_t split_mma<float, 64>(const DecodeArgs &, cudaStream_t, bool *) { return cudaErrorInvalidValue; }
-template <> cudaError_t split_mma<float, 256>(const DecodeArgs &, cudaStream_t, bool *) { return cudaErrorInvalidValue; }
+template <> cudaError_t split_mma<float, 128>(const DecodeArgs &, bool, cudaStream_t, bool *) { return cudaErrorInvalidValue; }   // never taken: 16-bit caches only
+template <> cudaError_t split_mma<float, 64>(const DecodeArgs &, bool, cudaStream_t, bool *) { return cudaErrorInvalidValue; }
+template <> cudaError_t split_mma<float, 256>(const DecodeArgs &, bool, cudaStream_t, bool *) { return cudaErrorInvalidValue; }
 
 // DASH_ATTN_DECODE_MMA=0 keeps the FMA pass (for comparison runs).
 static bool decode_force_scalar_pass() {
@@ -1231,20 +1245,19 @@ bool decode_fuses_rope(int dtype, const DecodeArgs &a, bool vector_ok) {
 
 // The split pass; *merged: it left the outputs, and no parts.
 template <typename T>
-static cudaError_t split_t(const DecodeArgs &a, bool vector_ok, cudaStream_t stream, bool *merged) {
+static cudaError_t split_t(const DecodeArgs &a, bool vector_ok, bool beside, cudaStream_t stream, bool *merged) {
     cudaError_t e;
     const bool mma = decode_uses_mma(sizeof(T), a, vector_ok);
-    if (mma && a.d == 128) e = split_mma<T, 128>(a, stream, merged);
-    else if (mma && a.d == 64) e = split_mma<T, 64>(a, stream, merged);
-    else if (mma && a.d == 256) e = split_mma<T, 256>(a, stream, merged);
-    else if (vector_ok && a.d == 64) e = split_vec<T, 64>(a, stream);
-    else if (vector_ok && a.d == 128) e = split_vec<T, 128>(a, stream);
-    else if (vector_ok && a.d == 256) e = split_vec<T, 256>(a, stream);
+    if (mma && a.d == 128) e = split_mma<T, 128>(a, beside, stream, merged);
+    else if (mma && a.d == 64) e = split_mma<T, 64>(a, beside, stream, merged);
+    else if (mma && a.d == 256) e = split_mma<T, 256>(a, beside, stream, merged);
+    else if (vector_ok && a.d == 64) e = split_vec<T, 64>(a, beside, stream);
+    else if (vector_ok && a.d == 128) e = split_vec<T, 128>(a, beside, stream);
+    else if (vector_ok && a.d == 256) e = split_vec<T, 256>(a, beside, stream);
     else {
         const long long units = (long long)a.splits * a.hq;
-        dim3 grid((unsigned)((units + DEC_WARPS - 1) / DEC_WARPS), a.b);
-        decode_split_scalar_kernel<T><<<grid, DEC_WARPS * 32, 0, stream>>>(a);
-        e = cudaGetLastError();
+        dim3 grid((unsigned)((units + DEC_WARPS - 1) / DEC_WARPS + beside), a.b);
+        e = launch_beside(beside ? decode_split_scalar_kernel<T, true> : decode_split_scalar_kernel<T, false>, grid, DEC_WARPS * 32, 0, stream, beside, a);
     }
     return e;
 }
@@ -1252,7 +1265,7 @@ static cudaError_t split_t(const DecodeArgs &a, bool vector_ok, cudaStream_t str
 template <typename T>
 static cudaError_t decode_t(const DecodeArgs &a, bool vector_ok, cudaStream_t stream, int *launches) {
     bool merged = false;
-    const cudaError_t e = split_t<T>(a, vector_ok, stream, &merged);
+    const cudaError_t e = split_t<T>(a, vector_ok, false, stream, &merged);
     *launches += 1;
     if (e != cudaSuccess || merged) return e;
     *launches += 1;
@@ -1282,12 +1295,12 @@ cudaError_t launch_decode(int dtype, const DecodeArgs &a, bool vector_ok, cudaSt
     }
 }
 
-cudaError_t launch_decode_parts(int dtype, const DecodeArgs &a, bool vector_ok, cudaStream_t stream, int *launches) {
+cudaError_t launch_decode_parts(int dtype, const DecodeArgs &a, bool vector_ok, bool beside, cudaStream_t stream, int *launches) {
     *launches += 1;
     switch (dtype) {
-        case 0: return split_t<float>(a, vector_ok, stream, nullptr);
-        case 1: return split_t<__nv_bfloat16>(a, vector_ok, stream, nullptr);
-        default: return split_t<__half>(a, vector_ok, stream, nullptr);
+        case 0: return split_t<float>(a, vector_ok, beside, stream, nullptr);
+        case 1: return split_t<__nv_bfloat16>(a, vector_ok, beside, stream, nullptr);
+        default: return split_t<__half>(a, vector_ok, beside, stream, nullptr);
     }
 }
 

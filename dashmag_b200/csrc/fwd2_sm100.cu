@@ -157,6 +157,8 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int hk = h0 / (a.hq / a.hkv);
     const int m_base = qt * NT * bt;
     auto tile_row0 = [&](int t) { return m_base + t * bt; };
+    // The block's second tile may hold no row (PREFIX: few sequences to a prompt): the first is then alone, and takes no turns.
+    const bool solo = PREFIX && tile_row0(1) >= a.tq;
     auto BAR = [&](uint64_t &x) { return smem_u32(&x); };
 
     if (threadIdx.x == 0) {
@@ -165,9 +167,9 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         mbar_init(BAR(sh.bar.q_full), 1);
         for (int i = 0; i < NS; ++i) {
             mbar_init(BAR(sh.bar.k_full[i]), 1);
-            mbar_init(BAR(sh.bar.k_empty[i]), NT);   // one commit per tile's issuer
+            mbar_init(BAR(sh.bar.k_empty[i]), solo ? 1 : NT);   // one commit per tile's issuer
             mbar_init(BAR(sh.bar.v_full[i]), 1);
-            mbar_init(BAR(sh.bar.v_empty[i]), NT);
+            mbar_init(BAR(sh.bar.v_empty[i]), solo ? 1 : NT);
         }
         for (int t = 0; t < NT; ++t) {
             for (int buf = 0; buf < 2; ++buf) {
@@ -301,7 +303,7 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         // fill it.  So each tile has an issuing warp of its own, on a scheduler of its own, whose waits fall
         // under the other tile's products.  The whole warp runs the (warp-uniform) code, so that barrier
         // addresses and descriptors are made in the uniform datapath; one elected lane issues.
-        if (subs > 0) {
+        if (subs > 0 && !(solo && warp == MMA_WARP1)) {
             const int t = __shfl_sync(0xffffffffu, warp, 0) == MMA_WARP0 ? 0 : 1;
             constexpr uint32_t IDESC_S = idesc_f16(BM, SN, Pack<T>::FMT, 0, 0);   // [128 q x 64 keys], A = Q, B = K K-major
             constexpr uint32_t IDESC_O = idesc_f16(BM, HD, Pack<T>::FMT, 0, 1);   // [128 q x HD], A = P (TMEM), B = V MN-major
@@ -390,7 +392,7 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             }
 #undef FWD2_BAR
         }
-    } else {
+    } else if (!(solo && tile == 1)) {
         // ---------------- softmax of one tile, one row per thread ----------------
         const int t = tile, h = h0 + (r & ((1 << pack) - 1));
         const int row = tile_row0(t) + (r >> pack);
@@ -482,7 +484,7 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             // u, then tile 1's, then tile 0's of u + 1 ..., each doing the rest of its sub-step (the wait for
             // S, the maximum, the store of P) under the other's turn.  (Bounded waits on barriers of the
             // block's own, like every other wait here; both tiles sweep the same sub-steps.)
-            if (t == 1 || u > 0) {
+            if (!solo && (t == 1 || u > 0)) {
                 if (!__all_sync(0xffffffffu, mbar_wait(BAR(sh.bar.turn[warp & 3][t]), (t == 1 ? u : u - 1) & 1))) { failed = true; break; }
             }
             // P over the first 32 columns of the buffer this thread has read (two 16-bit values a column).
@@ -500,7 +502,7 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 tmem_st16(t_lane + COL_S(t, buf) + cc * 16, pk);
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(BAR(sh.bar.turn[warp & 3][t ^ 1]));   // the other tile's turn
+            if (!solo && lane == 0) mbar_arrive(BAR(sh.bar.turn[warp & 3][t ^ 1]));   // the other tile's turn
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
@@ -615,18 +617,18 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         tc_fence_after_sync();
         tmem_dealloc(tmem, 512);
     }
-    if constexpr (PREFIX) end_beside();
 }
 
 namespace {
 template <typename T, int HD>
-cudaError_t launch_fwd2_prefix_t(dim3 grid, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Sm100FwdArgs &a, bool beside,
+cudaError_t launch_fwd2_prefix_t(dim3 grid, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Sm100FwdArgs &a,
                                  cudaStream_t stream) {
     constexpr size_t smem = Geo<HD>::SMEM_BYTES;
     const auto kernel = fwd2_sm100_kernel<T, HD, PREFIXES>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    return launch_beside(kernel, grid, THREADS, smem, stream, beside, tq, tk, tv, tq, a);   // (no output map: it leaves parts)
+    kernel<<<grid, THREADS, smem, stream>>>(tq, tk, tv, tq, a);   // (no output map: it leaves parts)
+    return cudaGetLastError();
 }
 template <typename T, int HD>
 cudaError_t launch_fwd2_t(dim3 grid, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const CUtensorMap &to,
@@ -652,14 +654,14 @@ cudaError_t launch_fwd2_sm100(int dtype, const CUtensorMap &tq, const CUtensorMa
 }
 
 cudaError_t launch_fwd2_prefix_sm100(int dtype, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Sm100FwdArgs &a,
-                                     bool beside, cudaStream_t stream) {
+                                     cudaStream_t stream) {
     const int tokens = (NT * BM) >> a.pack;   // per block
     dim3 grid(a.hq >> a.pack, (a.tq + tokens - 1) / tokens * a.splits, a.b);
     if (dtype == DASH_ATTN_BF16)
-        return a.d == 64 ? launch_fwd2_prefix_t<__nv_bfloat16, 64>(grid, tq, tk, tv, a, beside, stream)
-                         : launch_fwd2_prefix_t<__nv_bfloat16, 128>(grid, tq, tk, tv, a, beside, stream);
-    return a.d == 64 ? launch_fwd2_prefix_t<__half, 64>(grid, tq, tk, tv, a, beside, stream)
-                     : launch_fwd2_prefix_t<__half, 128>(grid, tq, tk, tv, a, beside, stream);
+        return a.d == 64 ? launch_fwd2_prefix_t<__nv_bfloat16, 64>(grid, tq, tk, tv, a, stream)
+                         : launch_fwd2_prefix_t<__nv_bfloat16, 128>(grid, tq, tk, tv, a, stream);
+    return a.d == 64 ? launch_fwd2_prefix_t<__half, 64>(grid, tq, tk, tv, a, stream)
+                     : launch_fwd2_prefix_t<__half, 128>(grid, tq, tk, tv, a, stream);
 }
 
 cudaError_t read_sm100_fwd2_status(unsigned int *status, bool clear) {

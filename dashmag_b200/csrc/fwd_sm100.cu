@@ -471,7 +471,6 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         tc_fence_after_sync();
         tmem_dealloc(tmem, 512);
     }
-    if constexpr (PREFIX) end_beside();
 }
 
 namespace {
@@ -486,22 +485,23 @@ cudaError_t launch_fwd_t(dim3 grid, const CUtensorMap &tq, const CUtensorMap &tk
     return cudaGetLastError();
 }
 template <typename T>
-cudaError_t launch_fwd_prefix_t(dim3 grid, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Sm100FwdArgs &a, bool beside,
+cudaError_t launch_fwd_prefix_t(dim3 grid, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Sm100FwdArgs &a,
                                 cudaStream_t stream) {
     constexpr size_t smem = Geo1<256>::SMEM_BYTES;
     const auto kernel = fwd_sm100_kernel<T, 256, PREFIXES>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    return launch_beside(kernel, grid, THREADS, smem, stream, beside, tq, tk, tv, a);
+    kernel<<<grid, THREADS, smem, stream>>>(tq, tk, tv, a);
+    return cudaGetLastError();
 }
 }  // namespace
 
 cudaError_t launch_fwd_prefix_sm100(int dtype, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Sm100FwdArgs &a,
-                                    bool beside, cudaStream_t stream) {
+                                    cudaStream_t stream) {
     const int tokens = BM >> a.pack;
     dim3 grid(a.hq >> a.pack, (a.tq + tokens - 1) / tokens * a.splits, a.b);
-    return dtype == DASH_ATTN_BF16 ? launch_fwd_prefix_t<__nv_bfloat16>(grid, tq, tk, tv, a, beside, stream)
-                                   : launch_fwd_prefix_t<__half>(grid, tq, tk, tv, a, beside, stream);
+    return dtype == DASH_ATTN_BF16 ? launch_fwd_prefix_t<__nv_bfloat16>(grid, tq, tk, tv, a, stream)
+                                   : launch_fwd_prefix_t<__half>(grid, tq, tk, tv, a, stream);
 }
 
 cudaError_t launch_fwd_sm100(int dtype, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv,

@@ -8,7 +8,8 @@
 // which all of the prompt's sequences are the rows of one product, each x group of them against every key-value head, so that a
 // prompt's keys are read from HBM once and not once per sequence: on the tensor cores the training forward's kernels take it
 // (fwd2_sm100.cu, fwd_sm100.cu, the prefix form; 16-bit, head dimension 64, 128 or 256), else the kernel here.
-// The passes touch nothing of one another: the second is launched beside the first, and the merge under its end.
+// The passes touch nothing of one another: that over the own keys, which HBM bounds, is launched beside the prompts', which is cut into no
+// more blocks than leave it multiprocessors (sm100_prefix_splits), and the merge under its end.
 #include <algorithm>
 
 #include "common.cuh"
@@ -139,7 +140,6 @@ __global__ void __launch_bounds__(THREADS) prefix_generic_kernel(PrefixArgs a) {
         for (int j = 0; j < MAX_D / 16; ++j)
             if (tx + 16 * j < a.d) a.part_o[at * a.d + tx + 16 * j] = acc[i][j] * inv;
     }
-    end_beside();
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -231,11 +231,12 @@ __global__ void __launch_bounds__(MERGE_THREADS) prefix_merge_kernel(PrefixMerge
 }
 
 template <typename T>
-cudaError_t generic_t(const PrefixArgs &a, dim3 grid, bool beside, cudaStream_t stream) {
+cudaError_t generic_t(const PrefixArgs &a, dim3 grid, cudaStream_t stream) {
     const size_t smem = generic_smem(a.d);
     cudaError_t e = cudaFuncSetAttribute(prefix_generic_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)generic_smem(MAX_D));
     if (e != cudaSuccess) return e;
-    return launch_beside(prefix_generic_kernel<T>, grid, THREADS, smem, stream, beside, a);
+    prefix_generic_kernel<T><<<grid, THREADS, smem, stream>>>(a);
+    return cudaGetLastError();
 }
 
 template <typename T>
@@ -258,15 +259,15 @@ int prefix_generic_splits(int n, int each, int p, int hq, int hkv) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(tiles, 2 * 148 / std::max<int64_t>(units, 1)));
 }
 
-cudaError_t launch_prefix_generic(int dtype, const PrefixArgs &a, bool beside, cudaStream_t stream, int *launches) {
+cudaError_t launch_prefix_generic(int dtype, const PrefixArgs &a, cudaStream_t stream, int *launches) {
     const int64_t x = generic_units(1, a.each, a.hq, a.hkv) * a.splits;
     if (x > 0x7fffffffLL) return cudaErrorInvalidValue;
     const dim3 grid((unsigned)x, (unsigned)a.n);
     *launches += 1;
     switch (dtype) {
-        case 0: return generic_t<float>(a, grid, beside, stream);
-        case 1: return generic_t<__nv_bfloat16>(a, grid, beside, stream);
-        default: return generic_t<__half>(a, grid, beside, stream);
+        case 0: return generic_t<float>(a, grid, stream);
+        case 1: return generic_t<__nv_bfloat16>(a, grid, stream);
+        default: return generic_t<__half>(a, grid, stream);
     }
 }
 

@@ -33,13 +33,14 @@ struct PrefixMergeArgs {
 
 // On the CUDA cores: any dtype, strides and head dimension up to 256.
 int prefix_generic_splits(int n, int each, int p, int hq, int hkv);
-cudaError_t launch_prefix_generic(int dtype, const PrefixArgs &a, bool beside, cudaStream_t stream, int *launches);
+cudaError_t launch_prefix_generic(int dtype, const PrefixArgs &a, cudaStream_t stream, int *launches);
 cudaError_t launch_prefix_merge(int dtype, const PrefixMergeArgs &a, cudaStream_t stream, int *launches);
 // On the tensor cores (sm100.cu): whether a call may run there as far as its shape says (0 splits: no), and, its pointers and strides
 // allowing, that it does.
-int sm100_prefix_splits(int dtype, float scale, int n, int each, int p, int hq, int hkv, int d);
+// `own_bytes`: what the pass over the sequences' own keys reads beside it.
+int sm100_prefix_splits(int dtype, float scale, int n, int each, int p, int hq, int hkv, int d, double own_bytes);
 bool sm100_prefix_takes(const PrefixArgs &a);
 // False: the driver refused a tensor map.
-bool sm100_prefix(int dtype, const PrefixArgs &a, bool beside, cudaStream_t stream, int *launches, cudaError_t *error);
+bool sm100_prefix(int dtype, const PrefixArgs &a, cudaStream_t stream, int *launches, cudaError_t *error);
 
 }  // namespace dash

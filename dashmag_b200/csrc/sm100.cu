@@ -328,17 +328,25 @@ cudaError_t sm100_forward(const dash_attn_params *p, const TrainArgs &a, void *w
     return e;
 }
 
-// The prompts' part of a decoding step over shared prompts.  Runs of keys a tile of rows: as forward_splits estimates, but that there is
-// a merge whatever the number, and that a call of many tiles needs none.
-int sm100_prefix_splits(int dtype, float scale, int n, int each, int p, int hq, int hkv, int d) {
+// The prompts' part of a decoding step over shared prompts: runs of keys a tile of rows is cut into.  Estimated in us, from forward_splits'
+// steps: a block's share of its sweep and what it costs however short that is, in waves; but the pass over the sequences' own
+// keys runs beside it, on the multiprocessors it leaves and then on all, so that what both cost of the GPU's time is a bound too; and the f32 rows
+// of the parts, written and read.
+int sm100_prefix_splits(int dtype, float scale, int n, int each, int p, int hq, int hkv, int d, double own_bytes) {
     if (dtype == DASH_ATTN_F32 || (d != 64 && d != 128 && d != 256) || !(scale > 0.f) || !std::isfinite(scale)) return 0;
     const bool one = d == 256;
     const int pack = pack_log2(hq / hkv, each);
-    const int64_t sequences = (one ? 128 : 256) >> pack, step = one ? 128 : 64, sms = 148, tiles = (each + sequences - 1) / sequences;
+    const int64_t sequences = (one ? 128 : 256) >> pack, keys = one ? 128 : 64, sms = 148, tiles = (each + sequences - 1) / sequences;
     if ((hq >> pack) > 65535 || n > 65535 || tiles > 65535) return 0;
-    const int64_t blocks = tiles * (hq >> pack) * n, l = (p + step - 1) / step, fixed = one ? 3 : 6;
-    const double part = (double)n * each * hq * d * sizeof(float) / (one ? 4.1e6 : 2.2e6);
-    auto cost = [&](int64_t s) { return (double)((blocks * s + sms - 1) / sms) * ((l + s - 1) / s + fixed) + s * part; };
+    const int64_t blocks = tiles * (hq >> pack) * n, l = (p + keys - 1) / keys;
+    const bool solo = !one && 2 * each <= sequences;
+    const double step = one ? 1.8 : solo ? 0.6 : 0.95, fixed = one ? 5.4 : 5.7, own = own_bytes / 6.5e6;
+    const double part = (double)n * each * hq * d * sizeof(float) / 2.3e6;
+    auto cost = [&](int64_t s) {
+        const double block = (l + s - 1) / s * step + fixed;
+        const double waves = (double)((blocks * s + sms - 1) / sms) * block, all = (double)blocks * s * block / sms + own;
+        return std::max(waves, all) + s * part;
+    };
     int best = 1;
     for (int s = 2; s <= 256 && s <= l && tiles * s <= 65535; ++s)
         if (cost(s) < cost(best)) best = s;
@@ -357,7 +365,7 @@ bool sm100_prefix_takes(const PrefixArgs &a) {
     const View4 q{a.q, a.q_sb * a.each, a.q_sb, a.q_sh, a.q_sd};
     return readable(q, a.n, a.each, a.hq) && readable(a.k, a.n, a.p, a.hkv) && readable(a.v, a.n, a.p, a.hkv) && device_is_sm100() && encoder();
 }
-bool sm100_prefix(int dtype, const PrefixArgs &a, bool beside, cudaStream_t stream, int *launches, cudaError_t *error) {
+bool sm100_prefix(int dtype, const PrefixArgs &a, cudaStream_t stream, int *launches, cudaError_t *error) {
     CUtensorMap tq, tk, tv;
     const int pack = pack_log2(a.hq / a.hkv, a.each);
     const int64_t qs[4] = {a.q_sb * a.each, a.q_sb, a.q_sh, a.q_sd}, ks[4] = {a.k.sb, a.k.st, a.k.sh, a.k.sd}, vs[4] = {a.v.sb, a.v.st, a.v.sh, a.v.sd};
@@ -374,7 +382,7 @@ bool sm100_prefix(int dtype, const PrefixArgs &a, bool beside, cudaStream_t stre
     f.part_lse = a.part_lse;
     f.reach = a.reach;
     *launches += 1;
-    *error = a.d == 256 ? launch_fwd_prefix_sm100(dtype, tq, tk, tv, f, beside, stream) : launch_fwd2_prefix_sm100(dtype, tq, tk, tv, f, beside, stream);
+    *error = a.d == 256 ? launch_fwd_prefix_sm100(dtype, tq, tk, tv, f, stream) : launch_fwd2_prefix_sm100(dtype, tq, tk, tv, f, stream);
     return true;
 }
 

@@ -69,11 +69,11 @@ cudaError_t launch_fwd_merge(int dtype, const Sm100FwdArgs &a, cudaStream_t stre
 cudaError_t launch_fwd_sm100(int dtype, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv,
                              const Sm100FwdArgs &a, cudaStream_t stream);
 // The prompts' part of a decoding step (prefix.cu): the forward's kernels over queries [N, sequences of a prompt, Hq, D] and keys
-// [N, P, Hkv, D], every block a part of its rows' keys.  `beside`: beside the launch in front of it.
+// [N, P, Hkv, D], every block a part of its rows' keys.
 cudaError_t launch_fwd_prefix_sm100(int dtype, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Sm100FwdArgs &a,
-                                    bool beside, cudaStream_t stream);
+                                    cudaStream_t stream);
 cudaError_t launch_fwd2_prefix_sm100(int dtype, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Sm100FwdArgs &a,
-                                     bool beside, cudaStream_t stream);
+                                     cudaStream_t stream);
 // The two-tile forward: tq with boxes of 128 rows, tk / tv with boxes of 64 rows.
 cudaError_t launch_fwd2_sm100(int dtype, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv,
                               const CUtensorMap &to, const Sm100FwdArgs &a, cudaStream_t stream);
