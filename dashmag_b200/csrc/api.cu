@@ -726,7 +726,7 @@ static int check_prefix(const char *op, const dash_attn_decode_params *p, const 
 
 // The parts of a call in the workspace: the prompts' (of as many runs as whichever kernels take it cut), then the own chunks'.
 struct PrefixSpace {
-    int tensor, generic, chunk, chunks;
+    int tensor, generic, chunk, chunks, own_tensor, own_generic;
     size_t part_o, part_lse, own_o, own_lse;   // bytes
 };
 static PrefixSpace prefix_space(const dash_attn_decode_params *p, const dash_attn_prefix_params *x) {
@@ -742,8 +742,11 @@ static PrefixSpace prefix_space(const dash_attn_decode_params *p, const dash_att
     s.part_lse = align256(sizeof(float) * rows * splits);
     if (p->s > 0) {
         decode_plan(p, &s.chunk, &s.chunks);
-        s.own_o = align256(sizeof(float) * rows * s.chunks * p->d);
-        s.own_lse = align256(sizeof(float) * rows * s.chunks);
+        s.own_tensor = dash::sm100_prefix_splits(p->dtype, scale_for(p->has_scale, p->scale, p->d), p->b, 1, p->s, p->hq, p->hkv, p->d, 0.);
+        s.own_generic = dash::prefix_generic_splits(p->b, 1, p->s, p->hq, p->hkv);
+        const size_t parts = (size_t)std::max(s.chunks, std::max(s.own_tensor, s.own_generic));
+        s.own_o = align256(sizeof(float) * rows * parts * p->d);
+        s.own_lse = align256(sizeof(float) * rows * parts);
     }
     return s;
 }
@@ -785,7 +788,7 @@ int dash_attn_decode_shared(const dash_attn_decode_params *p, const dash_attn_pr
     a.part_lse = reinterpret_cast<float *>(at + s.part_o);
     const int64_t none = (int64_t)x->p + p->s + 1;
     const int64_t left = p->has_window && p->window_left >= 0 && p->window_left < none ? p->window_left : none;
-    a.reach = dash::PrefixReach{x->lengths, p->lengths, x->lengths_elem_bytes, p->lengths_elem_bytes, x->p, p->s, append ? 1 : 0, (int)left};
+    a.reach = dash::PrefixReach{x->lengths, p->lengths, x->lengths_elem_bytes, p->lengths_elem_bytes, x->p, p->s, append ? 1 : 0, 0, (int)left};
 
     dash::DecodeArgs own{};
     own.b = p->b; own.s = p->s; own.hq = p->hq; own.hkv = p->hkv; own.d = p->d;
@@ -806,19 +809,34 @@ int dash_attn_decode_shared(const dash_attn_decode_params *p, const dash_attn_pr
 
     int launches = 0;
     cudaError_t e = cudaSuccess;
-    if (s.tensor > 0 && !g_force_generic.load() && dash::sm100_prefix_takes(a)) {
-        a.splits = s.tensor;
-        if (!dash::sm100_prefix(p->dtype, a, stream, &launches, &e)) return fail(DASH_ATTN_CUDA, "%s: the driver refused a TMA tensor map over the inputs", op);
-        g_probe[DASH_ATTN_PROBE_TENSOR_CORE_RUNS] += 1;
-    } else {
-        a.splits = s.generic;
-        e = dash::launch_prefix_generic(p->dtype, a, stream, &launches);
-        g_probe[DASH_ATTN_PROBE_GENERIC_RUNS] += 1;
+    bool refused = false;
+    auto sweep = [&](dash::PrefixArgs &x, int tensor, int generic) {
+        const bool cores = tensor > 0 && !g_force_generic.load() && dash::sm100_prefix_takes(x);
+        x.splits = cores ? tensor : generic;
+        if (!cores) e = dash::launch_prefix_generic(p->dtype, x, stream, &launches);
+        else if (!dash::sm100_prefix(p->dtype, x, stream, &launches, &e)) refused = true;
+        return cores;
+    };
+    const bool vectors = decode_vectors(p, q, k_new, v_new, k_cache, v_cache), own_swept = p->s > 0 && !vectors;
+    dash::PrefixArgs b = a;
+    if (own_swept && append) e = dash::launch_prefix_append(p->dtype, own, stream, &launches);
+    if (e == cudaSuccess) g_probe[sweep(a, s.tensor, s.generic) ? DASH_ATTN_PROBE_TENSOR_CORE_RUNS : DASH_ATTN_PROBE_GENERIC_RUNS] += 1;
+    if (e == cudaSuccess && !refused && own_swept) {
+        b.beside = 1;
+        b.n = p->b; b.each = 1; b.p = p->s;
+        b.k = own.k; b.v = own.v;
+        b.part_o = own.part_o; b.part_lse = own.part_lse;
+        b.reach = dash::PrefixReach{p->lengths, nullptr, p->lengths_elem_bytes, 0, p->s, 0, 0, append ? 1 : 0, own.left};
+        sweep(b, s.own_tensor, s.own_generic);
+    } else if (e == cudaSuccess && !refused && p->s > 0) {
+        e = dash::launch_decode_parts(p->dtype, own, true, true, stream, &launches);
     }
-    if (e == cudaSuccess && p->s > 0)
-        e = dash::launch_decode_parts(p->dtype, own, decode_vectors(p, q, k_new, v_new, k_cache, v_cache), true, stream, &launches);
+    if (refused) {
+        g_probe[DASH_ATTN_PROBE_KERNEL_LAUNCHES] += launches;
+        return fail(DASH_ATTN_CUDA, "%s: the driver refused a TMA tensor map over the inputs", op);
+    }
     if (e == cudaSuccess) {
-        const dash::PrefixMergeArgs m{(int64_t)p->b * p->hq, p->hq, p->d, a.splits, a.part_o, a.part_lse, own, out};
+        const dash::PrefixMergeArgs m{(int64_t)p->b * p->hq, p->hq, p->d, a.splits, a.part_o, a.part_lse, own, own_swept ? b.splits : 0, out};
         e = dash::launch_prefix_merge(p->dtype, m, stream, &launches);
     }
     g_probe[DASH_ATTN_PROBE_KERNEL_LAUNCHES] += launches;

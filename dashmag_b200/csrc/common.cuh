@@ -277,11 +277,12 @@ struct PrefixReach {
     int prompt_bytes, lengths_bytes;
     int p, s;              // the most that a prompt, that a sequence holds
     int append;            // 1: the step's own row comes on top of `lengths`
+    int prompt_append;     // the same of `prompt` (a sequence's own keys swept as if they were a prompt's)
     int left;              // clamped to p + s + 1 = no bound
 };
 __device__ __forceinline__ void prefix_bounds(const PrefixReach &r, int prompt, int64_t sequence, int &lo, int &hi) {
     hi = r.p;
-    if (r.prompt) hi = min(max(load_index(r.prompt, r.prompt_bytes, prompt), 0), r.p);
+    if (r.prompt) hi = (int)min((int64_t)max(load_index(r.prompt, r.prompt_bytes, prompt), 0) + r.prompt_append, (int64_t)r.p);
     int own = r.s;
     if (r.lengths) own = (int)min((int64_t)max(load_index(r.lengths, r.lengths_bytes, (int)sequence), 0) + r.append, (int64_t)r.s);
     lo = max(0, hi + own - 1 - r.left);

@@ -529,10 +529,11 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                     tmem_ld32(t_lane + COL_O(t) + c * 32, o);
                     tmem_ld_wait();
                     if (row < a.tq) {
-                        float4 *po = reinterpret_cast<float4 *>(a.part_o + at * HD + c * 32);
+                        // (PREFIX: heads of any multiple of eight features up to HD; the copies fill the others with zeros.)
+                        float4 *po = reinterpret_cast<float4 *>(a.part_o + at * (PREFIX ? a.d : HD) + c * 32);
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            po[e] = make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
+                            if (!PREFIX || c * 32 + 4 * e < a.d) po[e] = make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
                                                 __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
                     }
                 }
@@ -617,6 +618,7 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         tc_fence_after_sync();
         tmem_dealloc(tmem, 512);
     }
+    if constexpr (PREFIX) end_beside();
 }
 
 namespace {
@@ -627,8 +629,7 @@ cudaError_t launch_fwd2_prefix_t(dim3 grid, const CUtensorMap &tq, const CUtenso
     const auto kernel = fwd2_sm100_kernel<T, HD, PREFIXES>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    kernel<<<grid, THREADS, smem, stream>>>(tq, tk, tv, tq, a);   // (no output map: it leaves parts)
-    return cudaGetLastError();
+    return launch_beside(kernel, grid, THREADS, smem, stream, a.beside != 0, tq, tk, tv, tq, a);   // (no output map: it leaves parts)
 }
 template <typename T, int HD>
 cudaError_t launch_fwd2_t(dim3 grid, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const CUtensorMap &to,
@@ -658,9 +659,9 @@ cudaError_t launch_fwd2_prefix_sm100(int dtype, const CUtensorMap &tq, const CUt
     const int tokens = (NT * BM) >> a.pack;   // per block
     dim3 grid(a.hq >> a.pack, (a.tq + tokens - 1) / tokens * a.splits, a.b);
     if (dtype == DASH_ATTN_BF16)
-        return a.d == 64 ? launch_fwd2_prefix_t<__nv_bfloat16, 64>(grid, tq, tk, tv, a, stream)
+        return a.d <= 64 ? launch_fwd2_prefix_t<__nv_bfloat16, 64>(grid, tq, tk, tv, a, stream)
                          : launch_fwd2_prefix_t<__nv_bfloat16, 128>(grid, tq, tk, tv, a, stream);
-    return a.d == 64 ? launch_fwd2_prefix_t<__half, 64>(grid, tq, tk, tv, a, stream)
+    return a.d <= 64 ? launch_fwd2_prefix_t<__half, 64>(grid, tq, tk, tv, a, stream)
                      : launch_fwd2_prefix_t<__half, 128>(grid, tq, tk, tv, a, stream);
 }
 

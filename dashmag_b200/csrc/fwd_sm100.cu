@@ -429,10 +429,10 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                 tmem_ld32(t_lane + 256 + c * 32, o);
                 tmem_ld_wait();
                 if (row < a.tq && part) {
-                    float4 *po = reinterpret_cast<float4 *>(a.part_o + at * HD + c * 32);
+                    float4 *po = reinterpret_cast<float4 *>(a.part_o + at * (PREFIX ? a.d : HD) + c * 32);
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        po[e] = make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
+                        if (!PREFIX || c * 32 + 4 * e < a.d) po[e] = make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
                                             __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
                 } else if (row < a.tq) {
 #pragma unroll
@@ -471,6 +471,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         tc_fence_after_sync();
         tmem_dealloc(tmem, 512);
     }
+    if constexpr (PREFIX) end_beside();
 }
 
 namespace {
@@ -491,8 +492,7 @@ cudaError_t launch_fwd_prefix_t(dim3 grid, const CUtensorMap &tq, const CUtensor
     const auto kernel = fwd_sm100_kernel<T, 256, PREFIXES>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    kernel<<<grid, THREADS, smem, stream>>>(tq, tk, tv, a);
-    return cudaGetLastError();
+    return launch_beside(kernel, grid, THREADS, smem, stream, a.beside != 0, tq, tk, tv, a);
 }
 }  // namespace
 

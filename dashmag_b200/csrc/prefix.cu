@@ -7,7 +7,8 @@
 // sequences' own keys are those of the decoding step's split pass (decode.cu).  The parts over a prompt's keys come from a pass in
 // which all of the prompt's sequences are the rows of one product, each x group of them against every key-value head, so that a
 // prompt's keys are read from HBM once and not once per sequence: on the tensor cores the training forward's kernels take it
-// (fwd2_sm100.cu, fwd_sm100.cu, the prefix form; 16-bit, head dimension 64, 128 or 256), else the kernel here.
+// (fwd2_sm100.cu, fwd_sm100.cu, the prefix form; 16-bit, head dimensions of whole 16-byte vectors), else the kernel here.  Own keys that the
+// split pass could only read element by element are swept the same way, every sequence a prompt of one.
 // The passes touch nothing of one another: that over the own keys, which HBM bounds, is launched beside the prompts', which is cut into no
 // more blocks than leave it multiprocessors (sm100_prefix_splits), and the merge under its end.
 #include <algorithm>
@@ -25,74 +26,141 @@ namespace {
 // ---------------------------------------------------------------------------------------------
 // A block takes 32 rows (sequence, head) of a prompt's key-value head and a run of its keys, 64 at a time: queries, keys and then the
 // values of the same keys in shared memory as f32, scores and outputs in registers, two rows of four keys and of D / 16 features to a
-// thread, sixteen threads to a row.  f32 products and sums throughout, bound by the FMA pipe and its operands from shared memory.
+// thread, sixteen threads to a row.  The values are on their way to registers while the scores are made, the next keys while the outputs
+// are.  f32 products and sums throughout, bound by the FMA pipe and its operands from shared memory; with few rows by the trips to
+// memory (two prompts of 777 keys, three sequences each, 6 / 2 heads of 80 in f32: 41 us one element a load, waited for, now XX).
 constexpr int ROWS = 32, KEYS = 64, THREADS = 256, MAX_D = 256;
 
-size_t generic_smem(int d) { return sizeof(float) * ((size_t)ROWS * (d + 1) + (size_t)KEYS * (d + 1) + ROWS * (KEYS + 1)); }
+// Floats between rows of shared memory: whole 16-byte vectors, an odd number of them, so that eight rows' lie in banks of their own.
+__host__ __device__ constexpr int pitch_of(int d) { return 4 * (((d + 3) / 4) | 1); }
+size_t generic_smem(int d) { return sizeof(float) * ((size_t)(ROWS + KEYS) * pitch_of(d) + ROWS * (KEYS + 4)); }
 
-template <typename T>
+// 64 keys' rows on their way into shared memory, VE elements a load (16 bytes, or one element): up to AHEAD loads of a thread in registers,
+// what is more when they are put down.
+template <typename T, int VE> struct Rows {
+    static constexpr int AHEAD = VE > 1 ? 8 : 16;
+    struct alignas(VE > 1 ? 16 : sizeof(T)) Item { T e[VE]; };
+    Item held[AHEAD];
+    const T *base;   // the head's first key
+    int64_t st, sd;
+    int per, kmax;   // loads of a row; past the run's last key
+    __device__ __forceinline__ Rows(const View4 &v, int n, int hk, int d, int kmax)
+        : base(static_cast<const T *>(v.ptr) + (int64_t)n * v.sb + (int64_t)hk * v.sh), st(v.st), sd(v.sd), per(d / VE), kmax(kmax) {}
+    __device__ __forceinline__ Item load(int k0, int i) const {
+        const int k = i / per, c = (i - k * per) * VE;
+        Item x;
+        // (Keys past the run are zeros, whatever lies there.)
+        if (k < KEYS && k0 + k < kmax) {
+            const T *from = base + (int64_t)(k0 + k) * st + (int64_t)c * (VE > 1 ? 1 : sd);
+            if constexpr (VE > 1) *reinterpret_cast<uint4 *>(&x) = *reinterpret_cast<const uint4 *>(from);
+            else x.e[0] = *from;
+        } else {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) x.e[e] = Num<T>::from_f32(0.f);
+        }
+        return x;
+    }
+    __device__ __forceinline__ void ask(int k0) {
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a)
+            if (a * THREADS < KEYS * per) held[a] = load(k0, threadIdx.x + a * THREADS);
+    }
+    __device__ __forceinline__ void put(float *to, int pitch, int k0) {
+#pragma unroll 1
+        for (int i0 = 0; i0 < KEYS * per; i0 += AHEAD * THREADS) {
+            if (i0 > 0) {
+#pragma unroll
+                for (int a = 0; a < AHEAD; ++a) held[a] = load(k0, i0 + threadIdx.x + a * THREADS);
+            }
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                const int i = i0 + threadIdx.x + a * THREADS, k = i / per, c = (i - k * per) * VE;
+                if (k >= KEYS) break;
+                float *at = to + k * pitch + c;
+                if constexpr (VE == 1) {
+                    at[0] = Num<T>::to_f32(held[a].e[0]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VE; e += 4)
+                        *reinterpret_cast<float4 *>(at + e) = make_float4(Num<T>::to_f32(held[a].e[e]), Num<T>::to_f32(held[a].e[e + 1]),
+                                                                          Num<T>::to_f32(held[a].e[e + 2]), Num<T>::to_f32(held[a].e[e + 3]));
+                }
+            }
+        }
+    }
+};
+
+// VE: elements a load of keys and values; J: groups of 64 features, a quarter of a group to a thread.
+template <typename T, int VE, int J>
 __global__ void __launch_bounds__(THREADS) prefix_generic_kernel(PrefixArgs a) {
-    extern __shared__ float smem[];
-    __shared__ int row_lo[ROWS], row_hi[ROWS];
+    extern __shared__ float4 smem4[];
+    __shared__ int row_lo[ROWS], row_hi[ROWS], span[2];
     allow_beside();   // the merge
-    const int pitch = a.d + 1;
-    float *qs = smem, *ks = qs + ROWS * pitch, *ps = ks + KEYS * pitch;
+    const int pitch = pitch_of(a.d), d4 = (a.d + 3) / 4;
+    float *qs = reinterpret_cast<float *>(smem4), *ks = qs + ROWS * pitch, *ps = ks + KEYS * pitch;
     const int group = a.hq / a.hkv, split = blockIdx.x % a.splits, hk = blockIdx.x / a.splits % a.hkv;
     const int64_t r0 = (int64_t)(blockIdx.x / a.splits / a.hkv) * ROWS, rows = (int64_t)a.each * group;
     const int n = blockIdx.y, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
     auto sequence = [&](int64_t r) { return (int64_t)n * a.each + r / group; };
     auto head = [&](int64_t r) { return hk * group + (int)(r % group); };
 
+    static_assert(ROWS == 32, "a warp's lanes are the rows");
     if (threadIdx.x < ROWS) {
         int lo = a.p, hi = 0;
         const int64_t r = r0 + threadIdx.x;
         if (r < rows) prefix_bounds(a.reach, n, sequence(r), lo, hi);
         row_lo[threadIdx.x] = lo;
         row_hi[threadIdx.x] = hi;
+        lo = warp_min_i(hi > lo ? lo : a.p);
+        hi = warp_max_i(hi);
+        if (threadIdx.x == 0) { span[0] = lo; span[1] = hi; }
     }
-    for (int i = threadIdx.x; i < ROWS * a.d; i += THREADS) {
-        const int r = i / a.d, c = i - r * a.d;
-        qs[r * pitch + c] = r0 + r < rows ? Num<T>::to_f32(static_cast<const T *>(a.q)[sequence(r0 + r) * a.q_sb + head(r0 + r) * a.q_sh + c * a.q_sd]) : 0.f;
+    // (Columns behind the features, up to a whole vector: zeros, in the keys too, which are written but for them.)
+#pragma unroll 4
+    for (int i = threadIdx.x; i < ROWS * 4 * d4; i += THREADS) {
+        const int r = i / (4 * d4), c = i - r * 4 * d4;
+        qs[r * pitch + c] = r0 + r < rows && c < a.d ? Num<T>::to_f32(static_cast<const T *>(a.q)[sequence(r0 + r) * a.q_sb + head(r0 + r) * a.q_sh + c * a.q_sd]) : 0.f;
     }
+    if (a.d % 4 != 0)
+        for (int i = threadIdx.x; i < KEYS * 4; i += THREADS)
+            if (4 * (d4 - 1) + i % 4 >= a.d) ks[i / 4 * pitch + 4 * (d4 - 1) + i % 4] = 0.f;
     __syncthreads();
-    int kmin = a.p, kmax = 0;
-    for (int i = 0; i < ROWS; ++i) { kmin = min(kmin, row_hi[i] > row_lo[i] ? row_lo[i] : a.p); kmax = max(kmax, row_hi[i]); }
+    int kmin = span[0], kmax = span[1];
     split_keys(split, a.splits, KEYS, kmin, kmax);
 
-    float acc[2][MAX_D / 16], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float4 acc[2][J];
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < MAX_D / 16; ++j) acc[i][j] = 0.f;
-    // (Keys past the run are zeros, whatever lies there.)
-    auto fill = [&](const View4 &t, int k0) {
-        for (int i = threadIdx.x; i < KEYS * a.d; i += THREADS) {
-            const int k = i / a.d, c = i - k * a.d;
-            ks[k * pitch + c] = k0 + k < kmax ? load_f32<T>(t, n, k0 + k, hk, c) : 0.f;
-        }
-    };
+        for (int j = 0; j < J; ++j) acc[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    Rows<T, VE> keys(a.k, n, hk, a.d, kmax), values(a.v, n, hk, a.d, kmax);
+    const int lo0 = row_lo[2 * ty], lo1 = row_lo[2 * ty + 1], hi0 = row_hi[2 * ty], hi1 = row_hi[2 * ty + 1];
+    if (kmin < kmax) keys.ask(kmin);
     for (int k0 = kmin; k0 < kmax; k0 += KEYS) {
-        fill(a.k, k0);
+        keys.put(ks, pitch, k0);
         __syncthreads();
+        values.ask(k0);
         float s[2][4] = {};
-#pragma unroll 4
-        for (int c = 0; c < a.d; ++c) {
-            const float q0 = qs[(2 * ty) * pitch + c], q1 = qs[(2 * ty + 1) * pitch + c];
+        const float4 *q0 = reinterpret_cast<const float4 *>(qs + 2 * ty * pitch), *q1 = q0 + pitch / 4, *kk = reinterpret_cast<const float4 *>(ks + tx * pitch);
+#pragma unroll 2
+        for (int c = 0; c < d4; ++c) {
+            const float4 x = q0[c], y = q1[c];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float k = ks[(tx + 16 * j) * pitch + c];
-                s[0][j] = fmaf(q0, k, s[0][j]);
-                s[1][j] = fmaf(q1, k, s[1][j]);
+                const float4 k = kk[j * 4 * pitch + c];   // key tx + 16 j
+                s[0][j] = fmaf(x.x, k.x, fmaf(x.y, k.y, fmaf(x.z, k.z, fmaf(x.w, k.w, s[0][j]))));
+                s[1][j] = fmaf(y.x, k.x, fmaf(y.y, k.y, fmaf(y.z, k.z, fmaf(y.w, k.w, s[1][j]))));
             }
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int lo = row_lo[2 * ty + i], hi = row_hi[2 * ty + i];
+            const int lo = i ? lo1 : lo0, hi = i ? hi1 : hi0;
             float mx = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int key = k0 + tx + 16 * j;
-                s[i][j] = key >= lo && key < hi ? s[i][j] * a.scale : -INFINITY;
+                s[i][j] = key >= lo && key < hi && key < kmax ? s[i][j] * a.scale : -INFINITY;
                 mx = fmaxf(mx, s[i][j]);
             }
 #pragma unroll
@@ -103,27 +171,32 @@ __global__ void __launch_bounds__(THREADS) prefix_generic_kernel(PrefixArgs a) {
             for (int j = 0; j < 4; ++j) {
                 const float p = expf(s[i][j] - base);
                 sum += p;
-                ps[(2 * ty + i) * (KEYS + 1) + tx + 16 * j] = p;
+                ps[(2 * ty + i) * (KEYS + 4) + tx + 16 * j] = p;
             }
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             l[i] = l[i] * corr + sum;
             m[i] = mn;
 #pragma unroll
-            for (int j = 0; j < MAX_D / 16; ++j) acc[i][j] *= corr;
+            for (int j = 0; j < J; ++j) { acc[i][j].x *= corr; acc[i][j].y *= corr; acc[i][j].z *= corr; acc[i][j].w *= corr; }
         }
         __syncthreads();
-        fill(a.v, k0);
+        values.put(ks, pitch, k0);
         __syncthreads();
-        const int keys = min(KEYS, kmax - k0);
-        for (int k = 0; k < keys; ++k) {
-            const float p0 = ps[(2 * ty) * (KEYS + 1) + k], p1 = ps[(2 * ty + 1) * (KEYS + 1) + k];
+        if (k0 + KEYS < kmax) keys.ask(k0 + KEYS);
+        const int there = min(KEYS, kmax - k0);
+        const float *p0 = ps + 2 * ty * (KEYS + 4), *p1 = p0 + KEYS + 4;
+#pragma unroll 4
+        for (int k = 0; k < there; ++k) {
+            const float w0 = p0[k], w1 = p1[k];
 #pragma unroll
-            for (int j = 0; j < MAX_D / 16; ++j) {
-                if (tx + 16 * j >= a.d) break;
-                const float v = ks[k * pitch + tx + 16 * j];
-                acc[0][j] = fmaf(p0, v, acc[0][j]);
-                acc[1][j] = fmaf(p1, v, acc[1][j]);
+            for (int j = 0; j < J; ++j) {
+                if (tx + 16 * j >= d4) break;
+                const float4 v = *reinterpret_cast<const float4 *>(ks + k * pitch + 4 * (tx + 16 * j));
+                acc[0][j].x = fmaf(w0, v.x, acc[0][j].x); acc[0][j].y = fmaf(w0, v.y, acc[0][j].y);
+                acc[0][j].z = fmaf(w0, v.z, acc[0][j].z); acc[0][j].w = fmaf(w0, v.w, acc[0][j].w);
+                acc[1][j].x = fmaf(w1, v.x, acc[1][j].x); acc[1][j].y = fmaf(w1, v.y, acc[1][j].y);
+                acc[1][j].z = fmaf(w1, v.z, acc[1][j].z); acc[1][j].w = fmaf(w1, v.w, acc[1][j].w);
             }
         }
         __syncthreads();
@@ -136,10 +209,31 @@ __global__ void __launch_bounds__(THREADS) prefix_generic_kernel(PrefixArgs a) {
         // (A part that met a NaN leaves one: -inf is the mark of a part without keys.)
         if (tx == 0) a.part_lse[at] = l[i] != 0.f ? m[i] + logf(l[i]) : -INFINITY;
         const float inv = l[i] != 0.f ? 1.f / l[i] : 0.f;
+        float *po = a.part_o + at * a.d;
 #pragma unroll
-        for (int j = 0; j < MAX_D / 16; ++j)
-            if (tx + 16 * j < a.d) a.part_o[at * a.d + tx + 16 * j] = acc[i][j] * inv;
+        for (int j = 0; j < J; ++j) {
+            const int c = 4 * (tx + 16 * j);
+            if (c < a.d) po[c] = acc[i][j].x * inv;
+            if (c + 1 < a.d) po[c + 1] = acc[i][j].y * inv;
+            if (c + 2 < a.d) po[c + 2] = acc[i][j].z * inv;
+            if (c + 3 < a.d) po[c + 3] = acc[i][j].w * inv;
+        }
     }
+    end_beside();
+}
+
+// A warp a row of one cache.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) prefix_append_kernel(DecodeArgs a) {
+    const int64_t item = (int64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
+    if (item >= (int64_t)a.b * a.hkv * 2) return;
+    const bool is_v = item & 1;
+    const int b = (int)(item / 2 / a.hkv), hk = (int)(item / 2 % a.hkv), at = decode_append_at(a, b);
+    if (at < 0) return;
+    const View4 &to = is_v ? a.v : a.k;
+    const T *from = static_cast<const T *>(is_v ? a.v_new : a.k_new) + ((int64_t)b * a.hkv + hk) * a.d;
+    T *row = static_cast<T *>(const_cast<void *>(to.ptr)) + (int64_t)b * to.sb + (int64_t)at * to.st + (int64_t)hk * to.sh;
+    for (int c = threadIdx.x & 31; c < a.d; c += 32) row[(int64_t)c * to.sd] = from[c];
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -158,14 +252,16 @@ __global__ void __launch_bounds__(MERGE_THREADS) prefix_merge_kernel(PrefixMerge
     const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % WARPS, mine = (threadIdx.x >> 5) / WARPS;
     const int64_t row = (int64_t)blockIdx.x * AT_ONCE + mine;
     const bool live = row < a.rows;
-    int chunks = 0;
-    if (live && a.own.s > 0) {
+    int chunks = a.own_splits;
+    if (live && a.own.s > 0 && a.own_splits == 0) {
         int first, len;
         decode_range(a.own, (int)(row / a.hq), first, len);
         chunks = len > first ? (len - first + a.own.chunk - 1) / a.own.chunk : 0;   // those that hold keys
     }
     const int parts = live ? a.splits + chunks : 0;
-    auto lse_of = [&](int i) { return i < a.splits ? a.part_lse[i * a.rows + row] : a.own.part_lse[row * a.own.splits + i - a.splits]; };
+    // Where part i of the row lies, counted in rows of its array.
+    auto own_at = [&](int i) { return a.own_splits > 0 ? (int64_t)(i - a.splits) * a.rows + row : row * a.own.splits + i - a.splits; };
+    auto lse_of = [&](int i) { return i < a.splits ? a.part_lse[i * a.rows + row] : a.own.part_lse[own_at(i)]; };
     float top = -INFINITY;
     for (int i = lane * WARPS + warp; i < parts; i += 32 * WARPS) top = fmaxf(top, lse_of(i));
     top = warp_max(top);
@@ -183,10 +279,10 @@ __global__ void __launch_bounds__(MERGE_THREADS) prefix_merge_kernel(PrefixMerge
 #pragma unroll 4
     for (int i = warp; i < parts; i += WARPS) {
         const float lse = lse_of(i);
-        // A prompt's part that saw no key left nothing.  (A chunk of the sequence's own always left something; a NaN in it is one of the row.)
-        if (i < a.splits && lse == -INFINITY) continue;
+        // A run that saw no key left nothing.  (A chunk of the sequence's own always left something; a NaN in it is one of the row.)
+        if ((i < a.splits || a.own_splits > 0) && lse == -INFINITY) continue;
         const float w = expf(lse - top);
-        const float *po = i < a.splits ? a.part_o + (i * a.rows + row) * a.d : a.own.part_o + (row * a.own.splits + i - a.splits) * a.d;
+        const float *po = i < a.splits ? a.part_o + (i * a.rows + row) * a.d : a.own.part_o + own_at(i) * a.d;
         den += w;
         if (vec) {
 #pragma unroll
@@ -230,13 +326,24 @@ __global__ void __launch_bounds__(MERGE_THREADS) prefix_merge_kernel(PrefixMerge
     }
 }
 
+template <typename T, int VE, int J>
+cudaError_t generic_j(const PrefixArgs &a, dim3 grid, cudaStream_t stream) {
+    const auto kernel = prefix_generic_kernel<T, VE, J>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)generic_smem(64 * J));
+    if (e != cudaSuccess) return e;
+    return launch_beside(kernel, grid, THREADS, generic_smem(a.d), stream, a.beside != 0, a);
+}
+template <typename T, int VE>
+cudaError_t generic_v(const PrefixArgs &a, dim3 grid, cudaStream_t stream) {
+    return a.d <= 64 ? generic_j<T, VE, 1>(a, grid, stream) : a.d <= 128 ? generic_j<T, VE, 2>(a, grid, stream) : generic_j<T, VE, 4>(a, grid, stream);
+}
 template <typename T>
 cudaError_t generic_t(const PrefixArgs &a, dim3 grid, cudaStream_t stream) {
-    const size_t smem = generic_smem(a.d);
-    cudaError_t e = cudaFuncSetAttribute(prefix_generic_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)generic_smem(MAX_D));
-    if (e != cudaSuccess) return e;
-    prefix_generic_kernel<T><<<grid, THREADS, smem, stream>>>(a);
-    return cudaGetLastError();
+    constexpr int V = 16 / sizeof(T);
+    auto vectors = [&](const View4 &t) {
+        return reinterpret_cast<uintptr_t>(t.ptr) % 16 == 0 && t.sd == 1 && t.sb % V == 0 && t.st % V == 0 && t.sh % V == 0;
+    };
+    return a.d % V == 0 && vectors(a.k) && vectors(a.v) ? generic_v<T, V>(a, grid, stream) : generic_v<T, 1>(a, grid, stream);
 }
 
 template <typename T>
@@ -269,6 +376,16 @@ cudaError_t launch_prefix_generic(int dtype, const PrefixArgs &a, cudaStream_t s
         case 1: return generic_t<__nv_bfloat16>(a, grid, stream);
         default: return generic_t<__half>(a, grid, stream);
     }
+}
+
+cudaError_t launch_prefix_append(int dtype, const DecodeArgs &a, cudaStream_t stream, int *launches) {
+    const int64_t blocks = ((int64_t)a.b * a.hkv * 2 + THREADS / 32 - 1) / (THREADS / 32);
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+    *launches += 1;
+    if (dtype == 0) prefix_append_kernel<float><<<(unsigned)blocks, THREADS, 0, stream>>>(a);
+    else if (dtype == 1) prefix_append_kernel<__nv_bfloat16><<<(unsigned)blocks, THREADS, 0, stream>>>(a);
+    else prefix_append_kernel<__half><<<(unsigned)blocks, THREADS, 0, stream>>>(a);
+    return cudaGetLastError();
 }
 
 cudaError_t launch_prefix_merge(int dtype, const PrefixMergeArgs &a, cudaStream_t stream, int *launches) {

@@ -333,8 +333,9 @@ cudaError_t sm100_forward(const dash_attn_params *p, const TrainArgs &a, void *w
 // keys runs beside it, on the multiprocessors it leaves and then on all, so that what both cost of the GPU's time is a bound too; and the f32 rows
 // of the parts, written and read.
 int sm100_prefix_splits(int dtype, float scale, int n, int each, int p, int hq, int hkv, int d, double own_bytes) {
-    if (dtype == DASH_ATTN_F32 || (d != 64 && d != 128 && d != 256) || !(scale > 0.f) || !std::isfinite(scale)) return 0;
-    const bool one = d == 256;
+    // (Heads of a multiple of eight features: as 64, 128 or 256 with zeros behind them, which the copies bring.)
+    if (dtype == DASH_ATTN_F32 || d % 8 != 0 || d > 256 || !(scale > 0.f) || !std::isfinite(scale)) return 0;
+    const bool one = d > 128;
     const int pack = pack_log2(hq / hkv, each);
     const int64_t sequences = (one ? 128 : 256) >> pack, keys = one ? 128 : 64, sms = 148, tiles = (each + sequences - 1) / sequences;
     if ((hq >> pack) > 65535 || n > 65535 || tiles > 65535) return 0;
@@ -380,9 +381,10 @@ bool sm100_prefix(int dtype, const PrefixArgs &a, cudaStream_t stream, int *laun
     f.splits = a.splits;
     f.part_o = a.part_o;
     f.part_lse = a.part_lse;
+    f.beside = a.beside;
     f.reach = a.reach;
     *launches += 1;
-    *error = a.d == 256 ? launch_fwd_prefix_sm100(dtype, tq, tk, tv, f, stream) : launch_fwd2_prefix_sm100(dtype, tq, tk, tv, f, stream);
+    *error = a.d > 128 ? launch_fwd_prefix_sm100(dtype, tq, tk, tv, f, stream) : launch_fwd2_prefix_sm100(dtype, tq, tk, tv, f, stream);
     return true;
 }
 

@@ -74,8 +74,10 @@ DIMS = [
     (5, 1, 1, 1, 4, 2, 128),           # one key each
     (2, 7, 300, 20, 8, 2, 256),
     (1, 70, 65, 600, 4, 1, 256),
-    (2, 3, 777, 33, 6, 2, 80),         # on the CUDA cores whatever the dtype
-    (3, 2, 63, 5, 3, 3, 51),
+    (2, 3, 777, 33, 6, 2, 80),         # features that fill no tile
+    (2, 5, 200, 70, 8, 2, 136),
+    (3, 4, 150, 300, 4, 4, 24),
+    (3, 2, 63, 5, 3, 3, 51),           # on the CUDA cores whatever the dtype
     (1, 100, 200, 3, 10, 2, 32),
     (1, 1, 5000, 100, 32, 8, 128),     # one sequence, its prompt over the whole GPU
 ]
