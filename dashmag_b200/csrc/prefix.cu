@@ -239,90 +239,140 @@ __global__ void __launch_bounds__(THREADS) prefix_append_kernel(DecodeArgs a) {
 // ---------------------------------------------------------------------------------------------
 // The merge
 // ---------------------------------------------------------------------------------------------
-// WARPS warps a row, a lane up to four (D <= 128) or eight neighbouring features' worth of each part; the warps take the parts in turn and
-// meet in shared memory in their order, so the bits repeat.  Bound by launch and latency: the parts are in L2.
-constexpr int MERGE_THREADS = 128;
+// WARPS warps a row; LANES lanes a part (16 where a head is at most 64 features, else 32), four features or J times four each.  A lane asks for eight
+// parts' log-sum-exps and features at once, the first eight before it is known how many chunks the sequence's own keys make, and keeps
+// maximum, sum and outputs as the softmax does; the lanes' groups and the warps meet in order, so the bits repeat.
+// Bound by launch and latency, the parts being in L2: one trip to memory for most calls (one for the lengths, one for the log-sum-exps, one for the
+// parts: 2048 rows of 128 in five runs and up to eight chunks 9 us of a 45 us step, now XX).
+constexpr int MERGE_THREADS = 128, MERGE_EACH = 8;
 
-template <typename T, int WARPS>
+template <typename T, int WARPS, int LANES, int J>
 __global__ void __launch_bounds__(MERGE_THREADS) prefix_merge_kernel(PrefixMergeArgs a) {
-    constexpr int PER = MAX_D / 32, AT_ONCE = MERGE_THREADS / 32 / WARPS;   // rows of a block
-    __shared__ float red[AT_ONCE][WARPS][PER + 1][32];
-    __shared__ float tops[AT_ONCE][WARPS];
+    constexpr int AT_ONCE = MERGE_THREADS / 32 / WARPS, SUBS = 32 / LANES, STEP = WARPS * SUBS;   // rows of a block; groups of lanes; parts of a round
+    __shared__ float4 red[AT_ONCE][WARPS][J][32];
+    __shared__ float2 stat[AT_ONCE][WARPS][32];
     wait_before();   // the passes
     const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % WARPS, mine = (threadIdx.x >> 5) / WARPS;
+    const int slot = warp * SUBS + lane / LANES, col = lane % LANES;
     const int64_t row = (int64_t)blockIdx.x * AT_ONCE + mine;
-    const bool live = row < a.rows;
-    int chunks = a.own_splits;
-    if (live && a.own.s > 0 && a.own_splits == 0) {
+    const bool live = row < a.rows, vec = a.d % 4 == 0;
+    const bool chunked = a.own.s > 0 && a.own_splits == 0;   // the own keys' parts are the split pass's chunks
+    const int most = live ? a.splits + (chunked ? a.own.splits : a.own_splits) : 0;
+    // Where part i of the row lies, counted in rows of its array.
+    auto own_at = [&](int i) { return chunked ? row * a.own.splits + i - a.splits : (int64_t)(i - a.splits) * a.rows + row; };
+    float lse[MERGE_EACH];
+    float4 x[MERGE_EACH][J];
+    auto ask = [&](int i0, int end) {
+#pragma unroll
+        for (int e = 0; e < MERGE_EACH; ++e) {
+            const int i = i0 + e * STEP + slot;
+            lse[e] = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < J; ++j) x[e][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i >= end) continue;
+            const int64_t at = i < a.splits ? i * a.rows + row : own_at(i);
+            lse[e] = (i < a.splits ? a.part_lse : a.own.part_lse)[at];
+            const float *po = (i < a.splits ? a.part_o : a.own.part_o) + at * a.d;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int c = 4 * (col + LANES * j);
+                if (vec) {
+                    if (c < a.d) x[e][j] = *reinterpret_cast<const float4 *>(po + c);
+                } else {
+                    if (c < a.d) x[e][j].x = po[c];
+                    if (c + 1 < a.d) x[e][j].y = po[c + 1];
+                    if (c + 2 < a.d) x[e][j].z = po[c + 2];
+                    if (c + 3 < a.d) x[e][j].w = po[c + 3];
+                }
+            }
+        }
+    };
+    ask(0, most);
+    int parts = most;
+    if (live && chunked) {
         int first, len;
         decode_range(a.own, (int)(row / a.hq), first, len);
-        chunks = len > first ? (len - first + a.own.chunk - 1) / a.own.chunk : 0;   // those that hold keys
+        parts = a.splits + (len > first ? (len - first + a.own.chunk - 1) / a.own.chunk : 0);   // those that hold keys
     }
-    const int parts = live ? a.splits + chunks : 0;
-    // Where part i of the row lies, counted in rows of its array.
-    auto own_at = [&](int i) { return a.own_splits > 0 ? (int64_t)(i - a.splits) * a.rows + row : row * a.own.splits + i - a.splits; };
-    auto lse_of = [&](int i) { return i < a.splits ? a.part_lse[i * a.rows + row] : a.own.part_lse[own_at(i)]; };
-    float top = -INFINITY;
-    for (int i = lane * WARPS + warp; i < parts; i += 32 * WARPS) top = fmaxf(top, lse_of(i));
-    top = warp_max(top);
-    if constexpr (WARPS > 1) {
-        if (lane == 0) tops[mine][warp] = top;
-        __syncthreads();
+    float top = -INFINITY, den = 0.f;
+    float4 num[J];
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, tops[mine][w]);
-    }
-    if (top == -INFINITY) top = 0.f;
-    float num[PER], den = 0.f;
+    for (int j = 0; j < J; ++j) num[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    // Whether there is such a part: a run that saw no key left nothing.  (A chunk of the sequence's own always left something; a NaN in it is one of the row.)
+    auto there = [&](int i, float lse) { return i < parts && ((chunked && i >= a.splits) || lse != -INFINITY); };
+    auto scaled = [&](float by) {
+        den *= by;
 #pragma unroll
-    for (int c = 0; c < PER; ++c) num[c] = 0.f;
-    const bool vec = a.d % 4 == 0;   // features 4 lane + 128 j + (0..3), else lane + 32 j
-#pragma unroll 4
-    for (int i = warp; i < parts; i += WARPS) {
-        const float lse = lse_of(i);
-        // A run that saw no key left nothing.  (A chunk of the sequence's own always left something; a NaN in it is one of the row.)
-        if ((i < a.splits || a.own_splits > 0) && lse == -INFINITY) continue;
-        const float w = expf(lse - top);
-        const float *po = i < a.splits ? a.part_o + (i * a.rows + row) * a.d : a.own.part_o + own_at(i) * a.d;
-        den += w;
-        if (vec) {
+        for (int j = 0; j < J; ++j) { num[j].x *= by; num[j].y *= by; num[j].z *= by; num[j].w *= by; }
+    };
+    auto weight = [](float x, float top) { return expf(x - (top == -INFINITY ? 0.f : top)); };
+    for (int i0 = 0; i0 < parts; i0 += MERGE_EACH * STEP) {
+        if (i0 > 0) ask(i0, parts);
+        float now = top;
 #pragma unroll
-            for (int j = 0; j < PER / 4; ++j) {
-                const int c = 4 * lane + 128 * j;
-                if (c >= a.d) break;
-                const float4 x = *reinterpret_cast<const float4 *>(po + c);
-                num[4 * j] = fmaf(w, x.x, num[4 * j]);
-                num[4 * j + 1] = fmaf(w, x.y, num[4 * j + 1]);
-                num[4 * j + 2] = fmaf(w, x.z, num[4 * j + 2]);
-                num[4 * j + 3] = fmaf(w, x.w, num[4 * j + 3]);
-            }
-        } else {
+        for (int e = 0; e < MERGE_EACH; ++e)
+            if (there(i0 + e * STEP + slot, lse[e])) now = fmaxf(now, lse[e]);
+        scaled(weight(top, now));
+        top = now;
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                if (lane + 32 * j >= a.d) break;
-                num[j] = fmaf(w, po[lane + 32 * j], num[j]);
+        for (int e = 0; e < MERGE_EACH; ++e) {
+            if (!there(i0 + e * STEP + slot, lse[e])) continue;
+            const float w = weight(lse[e], top);
+            den += w;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                num[j].x = fmaf(w, x[e][j].x, num[j].x);
+                num[j].y = fmaf(w, x[e][j].y, num[j].y);
+                num[j].z = fmaf(w, x[e][j].z, num[j].z);
+                num[j].w = fmaf(w, x[e][j].w, num[j].w);
             }
         }
     }
-    if constexpr (WARPS > 1) {
+    auto join = [&](float o_top, float o_den, auto &&o_num) {
+        const float both = fmaxf(top, o_top), w = weight(o_top, both);
+        scaled(weight(top, both));
+        top = both;
+        den = fmaf(w, o_den, den);
 #pragma unroll
-        for (int c = 0; c < PER; ++c) red[mine][warp][c][lane] = num[c];
-        red[mine][warp][PER][lane] = den;
+        for (int j = 0; j < J; ++j) {
+            const float4 y = o_num(j);
+            num[j].x = fmaf(w, y.x, num[j].x);
+            num[j].y = fmaf(w, y.y, num[j].y);
+            num[j].z = fmaf(w, y.z, num[j].z);
+            num[j].w = fmaf(w, y.w, num[j].w);
+        }
+    };
+    if constexpr (SUBS == 2) {
+        const float o_top = __shfl_down_sync(0xffffffffu, top, 16), o_den = __shfl_down_sync(0xffffffffu, den, 16);
+        float4 o[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+            o[j] = make_float4(__shfl_down_sync(0xffffffffu, num[j].x, 16), __shfl_down_sync(0xffffffffu, num[j].y, 16),
+                               __shfl_down_sync(0xffffffffu, num[j].z, 16), __shfl_down_sync(0xffffffffu, num[j].w, 16));
+        join(o_top, o_den, [&](int j) { return o[j]; });   // (the upper lanes' own are of no use to anybody)
+    }
+    if constexpr (WARPS > 1) {
+        stat[mine][warp][lane] = make_float2(top, den);
+#pragma unroll
+        for (int j = 0; j < J; ++j) red[mine][warp][j][lane] = num[j];
         __syncthreads();
         if (warp != 0) return;
 #pragma unroll
         for (int w = 1; w < WARPS; ++w) {
-#pragma unroll
-            for (int c = 0; c < PER; ++c) num[c] += red[mine][w][c][lane];
-            den += red[mine][w][PER][lane];
+            const float2 o = stat[mine][w][lane];
+            join(o.x, o.y, [&](int j) { return red[mine][w][j][lane]; });
         }
     }
-    if (!live) return;
+    if (!live || lane >= LANES) return;
     const float inv = den != 0.f ? 1.f / den : 0.f;
     T *out = static_cast<T *>(a.out) + row * a.d;
 #pragma unroll
-    for (int c = 0; c < PER; ++c) {
-        const int f = vec ? 4 * lane + 128 * (c / 4) + c % 4 : lane + 32 * c;
-        if (f < a.d) out[f] = Num<T>::from_f32(num[c] * inv);
+    for (int j = 0; j < J; ++j) {
+        const int c = 4 * (col + LANES * j);
+        if (c < a.d) out[c] = Num<T>::from_f32(num[j].x * inv);
+        if (c + 1 < a.d) out[c + 1] = Num<T>::from_f32(num[j].y * inv);
+        if (c + 2 < a.d) out[c + 2] = Num<T>::from_f32(num[j].z * inv);
+        if (c + 3 < a.d) out[c + 3] = Num<T>::from_f32(num[j].w * inv);
     }
 }
 
@@ -346,14 +396,19 @@ cudaError_t generic_t(const PrefixArgs &a, dim3 grid, cudaStream_t stream) {
     return a.d % V == 0 && vectors(a.k) && vectors(a.v) ? generic_v<T, V>(a, grid, stream) : generic_v<T, 1>(a, grid, stream);
 }
 
+template <typename T, int WARPS>
+cudaError_t merge_w(const PrefixMergeArgs &a, cudaStream_t stream) {
+    constexpr int AT_ONCE = MERGE_THREADS / 32 / WARPS;
+    const int64_t blocks = (a.rows + AT_ONCE - 1) / AT_ONCE;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+    const auto kernel = a.d <= 64 ? prefix_merge_kernel<T, WARPS, 16, 1> : a.d <= 128 ? prefix_merge_kernel<T, WARPS, 32, 1> : prefix_merge_kernel<T, WARPS, 32, 2>;
+    return launch_beside(kernel, dim3((unsigned)blocks), MERGE_THREADS, 0, stream, true, a);
+}
+// Four warps a row where one would not have all parts on their way at once, and rows are few.
 template <typename T>
 cudaError_t merge_t(const PrefixMergeArgs &a, cudaStream_t stream) {
-    // Four warps a row where one would leave multiprocessors idle.
-    const bool few = a.rows <= 148 * 16;
-    const int at_once = MERGE_THREADS / 32 / (few ? 4 : 1);
-    const int64_t blocks = (a.rows + at_once - 1) / at_once;
-    if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-    return launch_beside(few ? prefix_merge_kernel<T, 4> : prefix_merge_kernel<T, 1>, dim3((unsigned)blocks), MERGE_THREADS, 0, stream, true, a);
+    const int parts = a.splits + (a.own.s > 0 ? std::max(a.own_splits, a.own_splits > 0 ? 0 : a.own.splits) : 0);
+    return parts > MERGE_EACH * (a.d <= 64 ? 2 : 1) && a.rows <= 148 * 16 ? merge_w<T, 4>(a, stream) : merge_w<T, 1>(a, stream);
 }
 
 int64_t generic_units(int n, int each, int hq, int hkv) { return (int64_t)n * hkv * (((int64_t)each * (hq / hkv) + ROWS - 1) / ROWS); }
