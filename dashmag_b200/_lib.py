@@ -245,7 +245,9 @@ _binding = None
 #: The functions the binding calls, in the order it takes them.
 BOUND = ("dash_attn_forward_workspace", "dash_attn_forward", "dash_attn_backward_workspace", "dash_attn_backward",
          "dash_attn_decode_workspace", "dash_attn_decode", "dash_attn_decode_append",
-         "dash_attn_decode_append_rope_workspace", "dash_attn_decode_append_rope", "dash_sample_workspace", "dash_sample")
+         "dash_attn_decode_append_rope_workspace", "dash_attn_decode_append_rope", "dash_sample_workspace", "dash_sample",
+         "dash_rope_norm_apply", "dash_rope_norm_backward_workspace", "dash_rope_norm_backward",
+         "dash_attn_decode_shared_workspace", "dash_attn_decode_shared", "dash_sample_penalize")
 
 
 class _Declines:

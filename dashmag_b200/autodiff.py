@@ -114,21 +114,21 @@ class QkNormNode(torch.autograd.Function):
     def forward(ctx, query, key, query_weight, key_weight, norm: QkNorm, where: dict):
         ctx.save_for_backward(query, key, query_weight, key_weight)
         ctx.norm, ctx.where = norm, where
-        return norm._forward(query, key, where)
+        return norm.forward_of(query, key, where)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_query, grad_key):
         query, key, query_weight, key_weight = ctx.saved_tensors
         norm = QkNorm(ctx.norm.rope, query_weight, key_weight, ctx.norm.eps)
-        grads = norm._backward(query, key, grad_query, grad_key, ctx.where)
+        grads = norm.backward_of(query, key, grad_query, grad_key, ctx.where)
         return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None)
 
 
 def _qk_norm(norm: QkNorm, query, key, where: dict):
     if _tracked(*(t for t in (query, key, norm.query_weight, norm.key_weight) if t is not None)):
         return QkNormNode.apply(query, key, norm.query_weight, norm.key_weight, norm, where)
-    return norm._forward(query, key, where)
+    return norm.forward_of(query, key, where)
 
 
 def qk_norm_range(norm: QkNorm, query, key, positions: range):

@@ -22,6 +22,7 @@
 #include <cmath>
 #include <cstdint>
 #include <cstring>
+#include <utility>
 
 #include "../../include/dash_attn.h"
 
@@ -40,12 +41,18 @@ struct Library {
     decltype(&dash_attn_decode_append_rope) decode_append_rope;
     decltype(&dash_sample_workspace) sample_workspace;
     decltype(&dash_sample) sample;
+    decltype(&dash_rope_norm_apply) norm_apply;
+    decltype(&dash_rope_norm_backward_workspace) norm_backward_workspace;
+    decltype(&dash_rope_norm_backward) norm_backward;
+    decltype(&dash_attn_decode_shared_workspace) decode_shared_workspace;
+    decltype(&dash_attn_decode_shared) decode_shared;
+    decltype(&dash_sample_penalize) penalize;
 } lib;
 
 // ---- what a call hands over ------------------------------------------------------------------------
 // The tensors a call's parameters point into that are not its arguments: an attribute may be a property whose tensor nobody else
 // holds, and what a mask or a Rope holds another thread may replace while the library is called without the interpreter's lock.
-using Held = c10::SmallVector<at::Tensor, 2>;
+using Held = c10::SmallVector<at::Tensor, 8>;
 
 struct Ref {   // an owned reference
     PyObject *p;
@@ -393,6 +400,170 @@ PyObject *decode_append_rope(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- the norm of queries and keys with the rotation ---------------------------------------------------
+struct Norm {
+    dash_rope_tables rope{};
+    dash_rope_norm_params p{};
+    const at::Tensor *q, *k, *g_q = nullptr, *g_k = nullptr, *w_q = nullptr, *w_k = nullptr;
+    Held held;
+};
+
+// A weight [d] of the tensors' dtype or f32; None: no weight.  False: not for us.
+bool norm_weight(PyObject *o, const Norm &n, const at::Tensor **out) {
+    if (o == Py_None) return true;
+    const at::Tensor *w = plain(o);
+    if (!w || w->dim() != 1 || w->size(0) != n.q->size(-1) || !w->is_contiguous() || w->get_device() != n.q->get_device()) return false;
+    if (w->scalar_type() != n.q->scalar_type() && w->scalar_type() != at::kFloat) return false;
+    *out = w;
+    return true;
+}
+
+// The call's arguments: args[0] the Rope, then query, key (and their gradients), the two weights, eps, and where the tokens are: 0 the positions
+// from `start` to `stop` of each sequence, 1 those of `index`, 2 packed by the offsets `index`, from `start` on.
+bool norm_call(Norm &n, PyObject *const *args, bool back) {
+    n.q = plain(args[1]);
+    n.k = plain(args[2]);
+    if (!n.q || !n.k) return false;
+    PyObject *const *rest = args + 3;
+    if (back) {
+        n.g_q = plain(rest[0]);
+        n.g_k = plain(rest[1]);
+        if (!n.g_q || !n.g_k) return false;
+        rest += 2;
+    }
+    const at::Tensor &q = *n.q, &k = *n.k;
+    int64_t form, start, stop;
+    if (!float_of(rest[2], &n.p.eps) || !int64_of(rest[3], &form) || !int64_of(rest[5], &start) || !int64_of(rest[6], &stop)) return false;
+    const int64_t rank = q.dim();
+    if (k.dim() != rank || (form == 0 ? rank != 4 : form == 1 ? rank != 3 : rank != 3 && rank != 4)) return false;
+    if (form == 2 && rank == 4 && (q.size(0) != 1 || k.size(0) != 1)) return false;
+    if (!fits32(q) || !fits32(k) || q.size(-1) != k.size(-1) || q.size(-3) != k.size(-3) || (rank == 4 && q.size(0) != k.size(0))) return false;
+    if (code_of(q.scalar_type()) < 0 || k.scalar_type() != q.scalar_type() || k.get_device() != q.get_device() || !on_current_device(q)) return false;
+    if (q.stride(-1) != 1 || k.stride(-1) != 1) return false;
+    if (!rope_tables(n.rope, n.held, args[0], q.scalar_type(), q.size(-1), q)) return false;
+    if (!norm_weight(rest[0], n, &n.w_q) || !norm_weight(rest[1], n, &n.w_k)) return false;
+    if (n.w_q && n.w_k && n.w_q->scalar_type() != n.w_k->scalar_type()) return false;
+    n.p.weight_dtype = code_of(n.w_q ? n.w_q->scalar_type() : n.w_k ? n.w_k->scalar_type() : q.scalar_type());
+    if (form == 0) {
+        if (stop - start != q.size(1) || start < 0 || stop > n.rope.len) return false;
+    } else {
+        const at::Tensor *index = plain(rest[4]);
+        if (!index || index->dim() != 1 || !fits32(*index) || !index->is_contiguous() || index->get_device() != q.get_device()) return false;
+        const int bytes = index_bytes(index->scalar_type());
+        if (bytes == 0 || index->size(0) < 1 || (form == 1 && index->size(0) != q.size(0))) return false;
+        if (form == 1) {
+            n.p.positions = index->data_ptr();
+            n.p.positions_elem_bytes = bytes;
+        } else {
+            n.p.cu_seqlens = index->data_ptr();
+            n.p.cu_seqlens_len = (int32_t)index->size(0);
+            n.p.index_elem_bytes = bytes;
+        }
+    }
+    n.p.start = start;
+    n.p.b = rank == 4 ? (int32_t)q.size(0) : 1;
+    n.p.t = q.size(-3);
+    n.p.d = (int32_t)q.size(-1);
+    n.p.heads_q = (int32_t)q.size(-2);
+    n.p.heads_k = (int32_t)k.size(-2);
+    auto strides3 = [&](int64_t *to, const at::Tensor &t) {
+        to[0] = rank == 4 ? t.stride(0) : 0;
+        to[1] = t.stride(-3);
+        to[2] = t.stride(-2);
+    };
+    strides3(n.p.q_stride, q);
+    strides3(n.p.k_stride, k);
+    if (back) {
+        for (const auto &[g, x] : {std::pair(n.g_q, n.q), std::pair(n.g_k, n.k)})
+            if (g->sizes() != x->sizes() || g->scalar_type() != x->scalar_type() || g->get_device() != x->get_device() || g->stride(-1) != 1) return false;
+        strides3(n.p.grad_q_stride, *n.g_q);
+        strides3(n.p.grad_k_stride, *n.g_k);
+    }
+    return true;
+}
+
+// norm(rope, query, key, query_weight, key_weight, eps, form, index, start, stop) -> (query, key)
+PyObject *norm(PyObject *, PyObject *const *args, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    Norm n;
+    if (count != 10 || !norm_call(n, args, false)) return nothing_done();
+    at::Tensor out_q, out_k;
+    const int rc = unlocked([&] {
+        out_q = fresh(n.q->sizes(), *n.q, n.q->scalar_type());
+        out_k = fresh(n.k->sizes(), *n.q, n.q->scalar_type());
+        return lib.norm_apply(&n.rope, &n.p, pointer(*n.q), pointer(*n.k), n.w_q ? pointer(*n.w_q) : nullptr, n.w_k ? pointer(*n.w_k) : nullptr, pointer(out_q),
+                              pointer(out_k), stream_of(*n.q));
+    });
+    if (rc != DASH_ATTN_OK) return PyLong_FromLong(rc);
+    return wrapped({out_q, out_k});
+    END_HANDLE_TH_ERRORS
+}
+
+// norm_backward(rope, query, key, grad_query, grad_key, query_weight, key_weight, eps, form, index, start, stop)
+//     -> (query, key, query_weight or None, key_weight or None)
+PyObject *norm_backward(PyObject *, PyObject *const *args, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    Norm n;
+    if (count != 12 || !norm_call(n, args, true)) return nothing_done();
+    at::Tensor dq, dk, dw_q, dw_k;
+    const int rc = unlocked([&] {
+        dq = fresh(n.q->sizes(), *n.q, n.q->scalar_type());
+        dk = fresh(n.k->sizes(), *n.q, n.q->scalar_type());
+        if (n.w_q) dw_q = fresh(n.w_q->sizes(), *n.q, n.w_q->scalar_type());
+        if (n.w_k) dw_k = fresh(n.w_k->sizes(), *n.q, n.w_k->scalar_type());
+        const size_t need = lib.norm_backward_workspace(&n.p);
+        at::Tensor ws = scratch(need, *n.q);
+        return lib.norm_backward(&n.rope, &n.p, pointer(*n.q), pointer(*n.k), n.w_q ? pointer(*n.w_q) : nullptr, n.w_k ? pointer(*n.w_k) : nullptr,
+                                 pointer(*n.g_q), pointer(*n.g_k), pointer(dq), pointer(dk), n.w_q ? pointer(dw_q) : nullptr, n.w_k ? pointer(dw_k) : nullptr,
+                                 need ? ws.data_ptr() : nullptr, need, stream_of(*n.q));
+    });
+    if (rc != DASH_ATTN_OK) return PyLong_FromLong(rc);
+    return wrapped({dq, dk, dw_q, dw_k});   // (None for a tensor that is none)
+    END_HANDLE_TH_ERRORS
+}
+
+// ---- decoding over shared prompts ----------------------------------------------------------------------
+// decode_shared(query, new_key, new_value, prefix_key, prefix_value, key, value, cache_lengths, prefix_lengths, options) -> out; no new rows: None
+PyObject *decode_shared(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 10) return nothing_done();
+    const at::Tensor *q = plain(args[0]), *pk = plain(args[3]), *pv = plain(args[4]), *k = plain(args[5]), *v = plain(args[6]);
+    const at::Tensor *nk = nullptr, *nv = nullptr;
+    dash_attn_decode_params p{};
+    dash_attn_prefix_params x{};
+    if (!q || !pk || !pv || !k || !v || !decode_params(p, *q, *k, *v, args[7], args[9])) return nothing_done();
+    if (args[1] != Py_None) {
+        nk = plain(args[1]);
+        nv = plain(args[2]);
+        if (args[7] == Py_None || !new_row(nk, *k) || !new_row(nv, *k)) return nothing_done();
+    }
+    for (const at::Tensor *t : {pk, pv})
+        if (t->dim() != 4 || !fits32(*t) || t->scalar_type() != q->scalar_type() || t->get_device() != q->get_device()) return nothing_done();
+    x.n = (int32_t)pk->size(0); x.p = (int32_t)pk->size(1); x.hkv = (int32_t)pk->size(2); x.d = (int32_t)pk->size(3);
+    x.v_n = (int32_t)pv->size(0); x.v_p = (int32_t)pv->size(1); x.v_hkv = (int32_t)pv->size(2); x.v_d = (int32_t)pv->size(3);
+    strides(x.k_stride, *pk);
+    strides(x.v_stride, *pv);
+    if (args[8] != Py_None) {
+        const at::Tensor *l = plain(args[8]);
+        if (!l || l->dim() != 1 || !fits32(*l) || !l->is_contiguous() || l->get_device() != q->get_device()) return nothing_done();
+        x.lengths_elem_bytes = index_bytes(l->scalar_type());
+        if (x.lengths_elem_bytes == 0) return nothing_done();
+        x.lengths = l->data_ptr();
+        x.lengths_len = (int32_t)l->size(0);
+    }
+    at::Tensor out;
+    const int rc = unlocked([&] {
+        out = fresh(q->sizes(), *q, q->scalar_type());
+        const size_t need = lib.decode_shared_workspace(&p, &x);
+        at::Tensor ws = scratch(need, *q);
+        return lib.decode_shared(&p, &x, pointer(*q), pointer(*pk), pointer(*pv), nk ? pointer(*nk) : nullptr, nv ? pointer(*nv) : nullptr, pointer(*k),
+                                 pointer(*v), pointer(out), need ? ws.data_ptr() : nullptr, need, stream_of(*q));
+    });
+    if (rc != DASH_ATTN_OK) return PyLong_FromLong(rc);
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
 // ---- sampling --------------------------------------------------------------------------------------
 bool attr_u64(PyObject *o, const char *name, uint64_t *out) {
     Ref v(PyObject_GetAttrString(o, name));
@@ -436,6 +607,99 @@ PyObject *sample(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// A penalty: a number, or f32 [b].  False: not for us.
+bool penalty_of(PyObject *rules, const char *name, const at::Tensor &z, bool history, float nothing, const float **each, float *all, Held &held) {
+    Ref o(PyObject_GetAttrString(rules, name));
+    if (!o.p) return false;
+    *all = nothing;
+    if (PyFloat_Check(o.p) || PyLong_Check(o.p)) return float_of(o.p, all) && (history || *all == nothing);
+    const at::Tensor *t = plain(o.p);
+    if (!t || t->dim() != 1 || t->size(0) != z.size(0) || t->scalar_type() != at::kFloat || !t->is_contiguous() || t->get_device() != z.get_device()) return false;
+    held.push_back(*t);
+    *each = static_cast<const float *>(pointer(*t));
+    return true;
+}
+// An attribute's tensor, on the logits' device; *out null for None.  False: not for us.
+bool tensor_of(PyObject *rules, const char *name, const at::Tensor &z, Held &held, const at::Tensor **out) {
+    Ref o(PyObject_GetAttrString(rules, name));
+    *out = nullptr;
+    if (!o.p) return false;
+    if (o.p == Py_None) return true;
+    const at::Tensor *t = plain(o.p);
+    if (!t || t->get_device() != z.get_device()) return false;
+    held.push_back(*t);
+    *out = &held.back();   // (the attribute may be a property's; eight are held where they are)
+    return true;
+}
+int64_t row_stride(const at::Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// penalize(logits, penalties) -> logits; into new ones
+PyObject *penalize(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 2) return nothing_done();
+    const at::Tensor *z = plain(args[0]);
+    PyObject *rules = args[1];
+    if (!z || z->dim() != 2 || !fits32(*z) || z->stride(1) != 1 || code_of(z->scalar_type()) < 0 || !on_current_device(*z)) return nothing_done();
+    dash_sample_penalize_params p{};
+    Held held;
+    p.dtype = code_of(z->scalar_type());
+    p.b = (int32_t)z->size(0);
+    p.v = (int32_t)z->size(1);
+    p.row_stride = row_stride(*z);
+    p.out_stride = p.v;
+    const at::Tensor *ids, *lengths, *prompt, *bias, *allowed;
+    if (!tensor_of(rules, "tokens", *z, held, &ids) || !tensor_of(rules, "lengths", *z, held, &lengths) || !tensor_of(rules, "prompt_lengths", *z, held, &prompt) ||
+        !tensor_of(rules, "bias", *z, held, &bias) || !tensor_of(rules, "allowed", *z, held, &allowed))
+        return nothing_done();
+    if (ids) {
+        p.ids_elem_bytes = index_bytes(ids->scalar_type());
+        if (p.ids_elem_bytes == 0 || ids->dim() != 2 || ids->size(0) != p.b || !fits32(*ids) || ids->stride(1) != 1) return nothing_done();
+        p.ids = pointer(*ids);
+        p.ids_len = (int32_t)ids->size(1);
+        p.ids_stride = row_stride(*ids);
+    } else if (lengths || prompt) {
+        return nothing_done();
+    }
+    for (const at::Tensor *t : {lengths, prompt})
+        if (t && (t->dim() != 1 || t->size(0) != p.b || !t->is_contiguous() || index_bytes(t->scalar_type()) == 0)) return nothing_done();
+    if (lengths) {
+        p.lengths = pointer(*lengths);
+        p.lengths_elem_bytes = index_bytes(lengths->scalar_type());
+    }
+    if (prompt) {
+        p.prompt_lengths = pointer(*prompt);
+        p.prompt_lengths_elem_bytes = index_bytes(prompt->scalar_type());
+    }
+    if (!penalty_of(rules, "repetition", *z, ids != nullptr, 1.f, &p.repetition, &p.repetition_all, held) ||
+        !penalty_of(rules, "frequency", *z, ids != nullptr, 0.f, &p.frequency, &p.frequency_all, held) ||
+        !penalty_of(rules, "presence", *z, ids != nullptr, 0.f, &p.presence, &p.presence_all, held))
+        return nothing_done();
+    if (bias) {
+        const bool rows = bias->dim() == 2;
+        if ((!rows && bias->dim() != 1) || bias->size(-1) != p.v || (rows && bias->size(0) != p.b) || bias->stride(-1) != 1) return nothing_done();
+        if (bias->scalar_type() != z->scalar_type() && bias->scalar_type() != at::kFloat) return nothing_done();
+        p.bias = pointer(*bias);
+        p.bias_dtype = code_of(bias->scalar_type());
+        p.bias_stride = rows ? row_stride(*bias) : 0;
+    }
+    if (allowed) {
+        const bool rows = allowed->dim() == 2;
+        const int64_t words = ((int64_t)p.v + 31) / 32;
+        if ((!rows && allowed->dim() != 1) || allowed->size(-1) != words || (rows && allowed->size(0) != p.b) || allowed->scalar_type() != at::kInt) return nothing_done();
+        if (allowed->stride(-1) != 1) return nothing_done();
+        p.allowed = pointer(*allowed);
+        p.allowed_stride = rows ? row_stride(*allowed) : 0;
+    }
+    at::Tensor out;
+    const int rc = unlocked([&] {
+        out = fresh(z->sizes(), *z, z->scalar_type());
+        return lib.penalize(&p, pointer(*z), pointer(out), stream_of(*z));
+    });
+    if (rc != DASH_ATTN_OK) return PyLong_FromLong(rc);
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
 // use(addresses): the library's functions, in Library's order
 PyObject *use(PyObject *, PyObject *const *args, Py_ssize_t n) {
     constexpr Py_ssize_t want = sizeof(Library) / sizeof(void *);
@@ -466,6 +730,10 @@ PyMethodDef methods[] = {
     {"decode_append", fast<decode_append>(), METH_FASTCALL, nullptr},
     {"decode_append_rope", fast<decode_append_rope>(), METH_FASTCALL, nullptr},
     {"sample", fast<sample>(), METH_FASTCALL, nullptr},
+    {"norm", fast<norm>(), METH_FASTCALL, nullptr},
+    {"norm_backward", fast<norm_backward>(), METH_FASTCALL, nullptr},
+    {"decode_shared", fast<decode_shared>(), METH_FASTCALL, nullptr},
+    {"penalize", fast<penalize>(), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -12,7 +12,7 @@ from typing import Any, Optional
 import torch
 
 from . import _lib
-from .attention import AttentionError, _check_device, _DTYPES, _index_bytes, _on, _ptr, _raise, _stream
+from .attention import AttentionError, _check_device, _DTYPES, _index_bytes, _on, _ptr, _raise, _result, _stream
 
 
 @dataclasses.dataclass(frozen=True)
@@ -41,6 +41,10 @@ class Penalties:
 def penalize(logits: torch.Tensor, penalties: Penalties, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``logits [B, V]`` (f32, bf16 or f16) under ``penalties``, f32 arithmetic rounded once; into ``out`` (which may be the logits) where
     given."""
+    if out is None:
+        done = _lib.binding().penalize(logits, penalties)
+        if done is not None:
+            return _result(done)
     op = "penalize"
     if logits.dim() != 2:
         raise AttentionError(f"{op}: logits must be [B, V], got {list(logits.shape)}")
@@ -84,7 +88,7 @@ def penalize(logits: torch.Tensor, penalties: Penalties, out: Optional[torch.Ten
             x = nothing
         elif x != nothing and tokens is None:
             raise AttentionError(f"{op}: a {name} penalty needs the tokens")
-        setattr(p, name + "_all", x)
+        setattr(p, name + "_all", float(x))
     bias = penalties.bias
     if bias is not None:
         if tuple(bias.shape) not in ((v,), (b, v)):

@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .attention import AttentionError, _check_device, _index_bytes, _on, _ptr, _raise, _stream, _workspace, make_decode_params
+from .attention import AttentionError, _check_device, _index_bytes, _on, _ptr, _raise, _result, _stream, _workspace, make_decode_params
 from .contract import AttentionOptions
 
 
@@ -70,6 +70,9 @@ def attention_decode_shared(query, prefix_key, prefix_value, key, value, cache_l
     ``N`` divides ``B`` and sequence ``b`` continues prompt ``b // (B // N)``.  ``key`` / ``value`` ``[B,S,Hkv,D]`` and ``cache_lengths [B]``
     as for ``attention_decode``.  Of the options the scale and the window's ``left`` apply, which counts over both.  What lies
     past the lengths may be anything."""
+    done = _lib.binding().decode_shared(query, None, None, prefix_key, prefix_value, key, value, cache_lengths, prefix_lengths, options)
+    if done is not None:
+        return _result(done)
     return _step("attention_decode_shared", query, None, None, prefix_key, prefix_value, key, value, cache_lengths, prefix_lengths, options)
 
 
@@ -78,6 +81,10 @@ def attention_decode_shared_append(query, new_key, new_value, prefix_key, prefix
     """The same step with the new rows ``[B,Hkv,D]`` written into the sequences' own caches first, at ``cache_lengths`` (the lengths
     before the step; a full cache gets no row), as ``attention_decode_append`` does."""
     op = "attention_decode_shared_append"
+    if new_key is not None and new_value is not None:
+        done = _lib.binding().decode_shared(query, new_key, new_value, prefix_key, prefix_value, key, value, cache_lengths, prefix_lengths, options)
+        if done is not None:
+            return _result(done)
     if cache_lengths is None:
         raise AttentionError(f"{op}: the lengths are needed: they say where each sequence's new row goes")
     if new_key is None or new_value is None:

@@ -14,8 +14,12 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .attention import AttentionError, _check_device, _DTYPES, _index_bytes, _on, _ptr, _raise, _stream, _workspace
+from .attention import AttentionError, _check_device, _DTYPES, _index_bytes, _on, _ptr, _raise, _result, _stream, _workspace
 from .rope import Rope
+
+
+# Where a call's tokens are, as the native host side takes it.
+_RANGE, _AT, _PACKED = 0, 1, 2
 
 
 class QkNormGradients(NamedTuple):
@@ -48,28 +52,50 @@ class QkNorm:
     # ------------------------------------------------------------------------------------------
     def apply_range(self, query: torch.Tensor, key: torch.Tensor, positions: range):
         """``query [B,T,Hq,D]`` and ``key [B,T,Hkv,D]`` at the positions ``positions`` of every sequence, ``T`` of them."""
+        if positions.step == 1:
+            done = _lib.binding().norm(self.rope, query, key, self.query_weight, self.key_weight, self.eps, _RANGE, None, positions.start, positions.stop)
+            if done is not None:
+                return _result(done)
         return self._forward(query, key, self._range(query, key, positions))
 
     def apply_at(self, query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor):
         """``query [B,Hq,D]`` and ``key [B,Hkv,D]``, one token per sequence, at ``positions [B]``, integer.  One outside the tables
         gives NaN in the rotated features, as ``Rope.apply_at`` does."""
+        done = _lib.binding().norm(self.rope, query, key, self.query_weight, self.key_weight, self.eps, _AT, positions, 0, 0)
+        if done is not None:
+            return _result(done)
         return self._forward(query, key, self._at(query, key, positions))
 
     def apply_packed(self, query: torch.Tensor, key: torch.Tensor, cu_seqlens: torch.Tensor, start: int = 0):
         """``[tokens,H,D]`` (or ``[1,tokens,H,D]``) of sequences packed back to back with the attention mask's offsets, every sequence
         from position ``start`` on; tokens of no sequence pass unchanged, neither normed nor rotated."""
+        done = _lib.binding().norm(self.rope, query, key, self.query_weight, self.key_weight, self.eps, _PACKED, cu_seqlens, start, 0)
+        if done is not None:
+            return _result(done)
         return self._forward(query, key, self._packed(query, key, cu_seqlens, start))
 
     def backward_range(self, query, key, grad_query, grad_key, positions: range) -> QkNormGradients:
         """The gradients of ``apply_range``'s inputs from those of its outputs."""
+        if positions.step == 1:
+            done = _lib.binding().norm_backward(self.rope, query, key, grad_query, grad_key, self.query_weight, self.key_weight, self.eps, _RANGE, None,
+                                                positions.start, positions.stop)
+            if done is not None:
+                return QkNormGradients(*_result(done))
         return self._backward(query, key, grad_query, grad_key, self._range(query, key, positions))
 
     def backward_at(self, query, key, grad_query, grad_key, positions: torch.Tensor) -> QkNormGradients:
         """The gradients of ``apply_at``'s inputs from those of its outputs."""
+        done = _lib.binding().norm_backward(self.rope, query, key, grad_query, grad_key, self.query_weight, self.key_weight, self.eps, _AT, positions, 0, 0)
+        if done is not None:
+            return QkNormGradients(*_result(done))
         return self._backward(query, key, grad_query, grad_key, self._at(query, key, positions))
 
     def backward_packed(self, query, key, grad_query, grad_key, cu_seqlens: torch.Tensor, start: int = 0) -> QkNormGradients:
         """The gradients of ``apply_packed``'s inputs from those of its outputs."""
+        done = _lib.binding().norm_backward(self.rope, query, key, grad_query, grad_key, self.query_weight, self.key_weight, self.eps, _PACKED, cu_seqlens,
+                                            start, 0)
+        if done is not None:
+            return QkNormGradients(*_result(done))
         return self._backward(query, key, grad_query, grad_key, self._packed(query, key, cu_seqlens, start))
 
     # ------------------------------------------------------------------------------------------
@@ -78,7 +104,7 @@ class QkNorm:
             raise AttentionError(f"Rope: positions {positions.start}..{positions.stop} of {len(self.rope)} for {list(query.shape)}")
         if key.dim() != 4 or key.shape[:2] != query.shape[:2]:
             raise AttentionError(f"Rope: {list(key.shape)} beside {list(query.shape)}")
-        return {"start": positions.start}
+        return {"start": positions.start, "stop": positions.stop}
 
     def _at(self, query, key, positions: torch.Tensor):
         if positions.dtype not in (torch.int32, torch.int64) or query.dim() != 3 or tuple(positions.shape) != (query.shape[0],):
@@ -130,6 +156,22 @@ class QkNorm:
             p.cu_seqlens, p.cu_seqlens_len, p.index_elem_bytes = _ptr(index), index.numel(), index.element_size()
         p.start = where.get("start", 0)
         return p, tensors, weights
+
+    @staticmethod
+    def _native(where):
+        """``where`` as the native host side takes it."""
+        form = _AT if "positions" in where else _PACKED if "cu_seqlens" in where else _RANGE
+        return form, where.get("positions", where.get("cu_seqlens")), where.get("start", 0), where.get("stop", 0)
+
+    def forward_of(self, query, key, where):
+        """The forward of a call that has been checked (``autodiff``'s node)."""
+        done = _lib.binding().norm(self.rope, query, key, self.query_weight, self.key_weight, self.eps, *self._native(where))
+        return _result(done) if done is not None else self._forward(query, key, where)
+
+    def backward_of(self, query, key, grad_query, grad_key, where):
+        """Its gradients."""
+        done = _lib.binding().norm_backward(self.rope, query, key, grad_query, grad_key, self.query_weight, self.key_weight, self.eps, *self._native(where))
+        return QkNormGradients(*_result(done)) if done is not None else self._backward(query, key, grad_query, grad_key, where)
 
     def _forward(self, query, key, where):
         p, (query, key), (wq, wk) = self._params("qk_norm", query, key, where)
