@@ -809,7 +809,7 @@ cudaError_t launch_qk_norm_backward(int dtype, const NormArgs &given, cudaStream
     cudaError_t e = run(dtype, a, p, true, stream);
     if (e != cudaSuccess || (!a.q.dw && !a.k.dw)) return e;
     *launches += 1;
-    const dim3 grid((unsigned)((a.d + 31) / 32), a.k.heads > 0 ? 2 : 1);
+    const dim3 grid((unsigned)((a.d + 31) / 32), 2);
     if (dtype == 0 || a.w_f32) return launch_beside(qk_norm_sum_kernel<float>, grid, THREADS, 0, stream, true, a, p.blocks_q, p.blocks);
     if (dtype == 1) return launch_beside(qk_norm_sum_kernel<__nv_bfloat16>, grid, THREADS, 0, stream, true, a, p.blocks_q, p.blocks);
     return launch_beside(qk_norm_sum_kernel<__half>, grid, THREADS, 0, stream, true, a, p.blocks_q, p.blocks);

@@ -2,7 +2,8 @@
 
 Bounds, u = 2^-24 and h the half step of the dtype (eps / 2): a sum of a head's squares is at most 25 additions deep, its root and the
 reciprocal four steps, the products and the sum of the rotation four: 32 u of the sum of the terms' magnitudes, and h of the result for the
-rounding.  The gradient has one more such sum: 64 u.  A weight's gradient is at most 256 additions deep at these sizes."""
+rounding.  The gradient has one more such sum: 64 u.  A weight's gradient is a sum
+of one lane's tokens and heads (at most 200 of them at these sizes, as twenty thousand tokens are dealt out), of its warps and blocks: 300 u."""
 import numpy as np
 import pytest
 import torch
@@ -195,6 +196,63 @@ def test_no_tokens():
     assert norm.apply_at(q, k, at)[0].shape == (0, 3, 32)
     g = norm.backward_at(q, k, q, k, at)
     assert g.query.shape == (0, 3, 32) and not g.query_weight.any() and not g.key_weight.any()
+
+
+@pytest.mark.parametrize("d", [64, 34])
+def test_a_tensor_without_heads(d):
+    """Its weight's gradient is an empty sum."""
+    t = torch.bfloat16
+    rope = make_rope(32, 64, t)
+    norm = QkNorm(rope, make((d,), t, 1), make((d,), t, 2))
+    q, none = make((20, 3, d), t, 3), make((20, 0, d), t, 4)
+    pos = torch.arange(20)
+    for a, b, x in ((q, none, 0), (none, q, 1)):
+        out = norm.apply_at(a, b, pos.to(DEV))
+        check_forward(out[x], q, (norm.query_weight, norm.key_weight)[x], rope, pos)
+        g = norm.backward_at(a, b, a, b, pos.to(DEV))
+        check_backward(g[x], g[2 + x], q, (norm.query_weight, norm.key_weight)[x], q, rope, pos)
+        assert not g[3 - x].any() and g[1 - x].numel() == 0
+
+
+@pytest.mark.parametrize("tokens,d", [(5, 64), (5, 34), (9000, 64)])
+def test_in_place_through_the_c_abi(tokens, d):
+    """Contiguous tensors may be their own results."""
+    import ctypes
+
+    t = torch.bfloat16
+    rope = make_rope(32, tokens, t)
+    q, k = make((1, tokens, 16, d), t, 3), make((1, tokens, 4, d), t, 4)
+    norm = QkNorm(rope)
+    want = norm.apply_range(q, k, range(tokens))
+    p, _, _ = norm._params("qk_norm", q, k, {"start": 0})
+    tables = rope.tables()
+    assert _lib.lib().dash_rope_norm_apply(ctypes.byref(tables), ctypes.byref(p), q.data_ptr(), k.data_ptr(), None, None, q.data_ptr(), k.data_ptr(),
+                                           torch.cuda.current_stream().cuda_stream) == _lib.OK
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+@pytest.mark.parametrize("dtype", list(TORCH))
+@pytest.mark.parametrize("hq,hkv,d,dim", [(32, 8, 128, 128), (16, 4, 64, 64), (8, 1, 64, 32), (5, 3, 96, 96), (70, 2, 32, 32), (12, 12, 256, 128)])
+def test_many_tokens(hq, hkv, d, dim, dtype):
+    """Long enough that every warp takes tokens one after another, several at a time where their heads are few, in sequences that end anywhere."""
+    t = TORCH[dtype]
+    n = 6007 if (hq + hkv) * d > 2000 else 20011
+    rope = make_rope(dim, n, t)
+    norm = QkNorm(rope, make((d,), t, 1), make((d,), t, 2))
+    q, k, gq, gk = (make((n, h, d), t, s) for s, h in enumerate((hq, hkv, hq, hkv)))
+    cu = [3, 3, 1000, 1001, 2500, n - 5]
+    args = torch.tensor(cu, dtype=torch.int32, device=DEV)
+    pos = torch.cat([torch.arange(b - a) for a, b in zip(cu, cu[1:])])
+    oq, ok = norm.apply_packed(q, k, args)
+    rows = slice(cu[0], cu[-1])
+    check_forward(oq[rows], q[rows], norm.query_weight, rope, pos)
+    check_forward(ok[rows], k[rows], norm.key_weight, rope, pos)
+    g = norm.backward_packed(q, k, gq, gk, args)
+    check_backward(g.query[rows], g.query_weight, q[rows], norm.query_weight, gq[rows], rope, pos)
+    check_backward(g.key[rows], g.key_weight, k[rows], norm.key_weight, gk[rows], rope, pos)
+    for rows in (slice(0, cu[0]), slice(cu[-1], n)):
+        assert torch.equal(oq[rows], q[rows]) and torch.equal(g.key[rows], gk[rows])
+    assert _lib.lib().dash_attn_device_status(0) == 0
 
 
 def test_zeros_and_large_heads():
