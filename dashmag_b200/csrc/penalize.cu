@@ -14,7 +14,7 @@
 // The history is read once per piece, from L2, so pieces are long - counters of 16 bits where no history overflows them - as far as the
 // blocks still fill the GPU evenly (chunks_of).  The pass is a read and a write of the logits, bound by HBM.
 // (Pieces of 8192 tokens held in registers, counters of 32 bits, four trips one after another: 256 rows of 100003 tokens with up to 8192
-// ids 85 us, one trip 58, now 38; clusters of eight blocks that read a share of the history each and count for one another in
+// ids 85 us, one trip 58, now 42; clusters of eight blocks that read a share of the history each and count for one another in
 // distributed shared memory 107: half of a text's ids are a few tokens, whose words all eight then wait for.)
 #include <algorithm>
 #include <type_traits>
@@ -25,7 +25,7 @@
 namespace dash {
 namespace {
 
-constexpr int THREADS = 512, DEPTH = 2;
+constexpr int THREADS = 256, BLOCKS = 5, DEPTH = 2;   // (blocks of a multiprocessor)
 
 // Counters of tokens: bits, the mark of a prompt's token, the count.
 template <typename C> struct Counter {
@@ -63,7 +63,7 @@ constexpr int AHEAD = 4;   // ids of a thread on their way at once
 
 // A block a piece of `chunks` times THREADS * V places.  I: the ids' integers, C: the counters'.
 template <typename T, typename I, typename C>
-__global__ void __launch_bounds__(THREADS, 2) penalize_kernel(PenalizeArgs a, int pieces, int chunks) {
+__global__ void __launch_bounds__(THREADS, BLOCKS) penalize_kernel(PenalizeArgs a, int pieces, int chunks) {
     constexpr int V = 16 / sizeof(T), CHUNK = THREADS * V, WORDS = V * sizeof(C) / 4;
     extern __shared__ uint4 smem[];
     unsigned *words = reinterpret_cast<unsigned *>(smem);
@@ -79,16 +79,14 @@ __global__ void __launch_bounds__(THREADS, 2) penalize_kernel(PenalizeArgs a, in
 
     const I *ids = static_cast<const I *>(a.ids) + (int64_t)row * a.ids_stride;
     I id[AHEAD];
-    int64_t length = 0, prompt_length = 0;
+    int64_t length, prompt_length;
     auto ask = [&](int i0, int end) {
 #pragma unroll
         for (int e = 0; e < AHEAD; ++e) id[e] = i0 + e * THREADS < end ? ids[i0 + e * THREADS] : I(-1);
     };
-    if (a.ids) {
-        length = number(a.lengths, a.lengths_bytes, row, a.t);
-        prompt_length = number(a.prompt, a.prompt_bytes, row, 0);
-        ask(threadIdx.x, a.t);
-    }
+    length = number(a.lengths, a.lengths_bytes, row, a.t);
+    prompt_length = number(a.prompt, a.prompt_bytes, row, 0);
+    ask(threadIdx.x, a.t);
     Rules r;
     r.repetition = a.repetition ? a.repetition[row] : a.repetition_all;
     r.inverse = 1.f / r.repetition;
@@ -110,10 +108,10 @@ __global__ void __launch_bounds__(THREADS, 2) penalize_kernel(PenalizeArgs a, in
     const int v_first = first + (int)threadIdx.x * V;
 #pragma unroll
     for (int j = 0; j < DEPTH; ++j) fetch(v_first + j * CHUNK, x[j], open[j], open2[j]);
-    if (a.ids) {
+    const int len = within(length, a.t), prompt = within(prompt_length, len);
+    if (len > 0) {
         for (int i = threadIdx.x; i < places / (4 * Counter<C>::PER); i += THREADS) smem[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        const int len = within(length, a.t), prompt = within(prompt_length, len);
         for (int i0 = threadIdx.x; i0 < len; i0 += THREADS * AHEAD) {
             if (i0 >= THREADS * AHEAD) ask(i0, len);
 #pragma unroll
@@ -135,7 +133,9 @@ __global__ void __launch_bounds__(THREADS, 2) penalize_kernel(PenalizeArgs a, in
     };
     auto pass = [&](int v0, const Vec<T, V> &x, uint32_t bits) {
         alignas(16) unsigned w[WORDS];
-        if (a.ids) {
+#pragma unroll
+        for (int e = 0; e < WORDS; ++e) w[e] = 0;
+        if (len > 0) {
             const unsigned *at = words + (v0 - first) / Counter<C>::PER;
 #pragma unroll
             for (int e = 0; e < WORDS; e += WORDS < 4 ? 2 : 4) {
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(THREADS, 2) penalize_kernel(PenalizeArgs a, in
                 const int v = v0 + e;
                 if (v < 0 || v >= a.v) continue;
                 float z = Num<T>::to_f32(in[v]);
-                if (a.ids) z = ruled<C>(r, z, Counter<C>::get(w, e));
+                z = ruled<C>(r, z, Counter<C>::get(w, e));
                 if (a.bias) z += bias_at(v);
                 if (allowed && !(allowed[v >> 5] >> (v & 31) & 1u)) z = -INFINITY;
                 out[v] = Num<T>::from_f32(z);
@@ -159,9 +159,9 @@ __global__ void __launch_bounds__(THREADS, 2) penalize_kernel(PenalizeArgs a, in
         float z[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) z[e] = Num<T>::to_f32(x.e[e]);
-        if (a.ids) {
-            // (All of a vector or nothing: a history of some thousands touches one vector in ten, nearly every warp's 32 of them.  Word by
-            // word the branches cost more than they spare, 256 rows of 100003 with up to 8192 ids 38.1 us against 42.8.)
+        if (len > 0) {
+            // (All of a vector or nothing: a history of some thousands touches one vector in ten, nearly every warp's 32 of them; word by word the
+            // branches cost what they spare.)
             unsigned any = 0;
 #pragma unroll
             for (int i = 0; i < WORDS; ++i) any |= w[i];
@@ -205,16 +205,92 @@ __global__ void __launch_bounds__(THREADS, 2) penalize_kernel(PenalizeArgs a, in
     }
 }
 
-constexpr int MOST_BYTES = 96 * 1024;   // of counters: two blocks a multiprocessor
+// ---------------------------------------------------------------------------------------------
+// Calls without a history
+// ---------------------------------------------------------------------------------------------
+// The bias and the grammar alone.  EACH vectors a thread, all asked for at once, a block as long as they take: nothing is counted, and nobody
+// waits for anybody (256 rows of 100003 tokens in bf16 18 us, 5.8 TB/s, where the kernel above takes 26 for histories of one id).
+// (Rows with short histories this way too, with their ids' logits made in a kernel beside it and put over its results: 25 us against 30 at 512
+// ids a row, but 29 against 32 at 2048, 44 against 41 at 8192, and 5.7 against 3.3 for one row of 32768.)
+template <typename T, int EACH>
+__global__ void __launch_bounds__(THREADS) penalize_all_kernel(PenalizeArgs a, int pieces) {
+    constexpr int V = 16 / sizeof(T), PIECE = THREADS * EACH * V;
+    const int row = blockIdx.x / pieces, piece = blockIdx.x - row * pieces;
+    const T *in = static_cast<const T *>(a.logits) + (int64_t)row * a.stride;
+    T *out = static_cast<T *>(a.out) + (int64_t)row * a.out_stride;
+    const int skew = (int)((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));
+    const bool vec = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+    const int first = piece * PIECE - skew;
+    const uint32_t *allowed = a.allowed ? a.allowed + (int64_t)row * a.allowed_stride : nullptr;
+    const int64_t bias0 = (int64_t)row * a.bias_stride;
+    auto token = [&](int j) { return first + (j * THREADS + (int)threadIdx.x) * V; };
+    auto whole = [&](int v0) { return vec && v0 >= 0 && v0 <= a.v - V; };
+    auto bias_at = [&](int v) {
+        return a.bias_f32 ? static_cast<const float *>(a.bias)[bias0 + v] : Num<T>::to_f32(static_cast<const T *>(a.bias)[bias0 + v]);
+    };
+    Vec<T, V> x[EACH];
+    uint32_t open[EACH], open2[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+        const int v0 = token(j);
+        if (!whole(v0)) continue;
+        *reinterpret_cast<uint4 *>(&x[j]) = *reinterpret_cast<const uint4 *>(in + v0);
+        if (allowed) {
+            open[j] = allowed[v0 >> 5];
+            if (skew) open2[j] = allowed[(v0 + V - 1) >> 5];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+        const int v0 = token(j);
+        if (!whole(v0)) {   // the row's ends
+            for (int v = max(v0, 0); v < min(v0 + V, a.v); ++v) {
+                float z = Num<T>::to_f32(in[v]);
+                if (a.bias) z += bias_at(v);
+                if (allowed && !(allowed[v >> 5] >> (v & 31) & 1u)) z = -INFINITY;
+                out[v] = Num<T>::from_f32(z);
+            }
+            continue;
+        }
+        if (a.bias || allowed) {
+            float z[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) z[e] = Num<T>::to_f32(x[j].e[e]);
+            if (a.bias) {
+                const bool four = a.bias_f32 && (reinterpret_cast<uintptr_t>(static_cast<const float *>(a.bias) + bias0 + v0) & 15) == 0;
+                if (four) {
+#pragma unroll
+                    for (int e = 0; e < V; e += 4) {
+                        const float4 b = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.bias) + bias0 + v0 + e);
+                        z[e] += b.x; z[e + 1] += b.y; z[e + 2] += b.z; z[e + 3] += b.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) z[e] += bias_at(v0 + e);
+                }
+            }
+            if (allowed) {
+                const uint32_t bits = skew ? __funnelshift_r(open[j], open2[j], v0 & 31) : open[j] >> (v0 & 31);
+#pragma unroll
+                for (int e = 0; e < V; ++e) z[e] = bits >> e & 1u ? z[e] : -INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[j].e[e] = Num<T>::from_f32(z[e]);
+        }
+        *reinterpret_cast<uint4 *>(out + v0) = *reinterpret_cast<const uint4 *>(&x[j]);
+    }
+}
 
-// Chunks of a piece.  The blocks run in waves of two a multiprocessor; a block costs its chunks, and about three and a half of them until
+constexpr int MOST_BYTES = 40 * 1024;   // of counters
+
+// Chunks of a piece.  The blocks run in waves of five a multiprocessor; a block costs its chunks, and about three and a half of them until
 // its first is there, and the history.
 int chunks_of(int64_t chunks_of_row, int b, int t, int most) {
     int best = 1;
     double least = 0.;
     for (int k = 1; k <= most; ++k) {
-        const int64_t blocks = (chunks_of_row + k - 1) / k * b, waves = (blocks + 2 * 148 - 1) / (2 * 148);
-        const double cost = waves * (k + 3.5 + t / 3000.);
+        const int64_t blocks = (chunks_of_row + k - 1) / k * b, waves = (blocks + BLOCKS * 148 - 1) / (BLOCKS * 148);
+        const double cost = waves * (k + 3.5 + t / 1500.);
         if (k == 1 || cost < least) { best = k; least = cost; }
         if (k >= chunks_of_row) break;
     }
@@ -225,20 +301,27 @@ template <typename T, typename I, typename C>
 cudaError_t run(const PenalizeArgs &a, cudaStream_t stream) {
     constexpr int CHUNK = THREADS * 16 / (int)sizeof(T);
     const int64_t row = ((int64_t)a.v + 16 / (int)sizeof(T) - 1 + CHUNK - 1) / CHUNK;
-    const int chunks = chunks_of(row, a.b, a.ids ? a.t : 0, MOST_BYTES / (CHUNK * (int)sizeof(C)));
+    const int chunks = chunks_of(row, a.b, a.t, MOST_BYTES / (CHUNK * (int)sizeof(C)));
     const int64_t pieces = (row + chunks - 1) / chunks, blocks = pieces * a.b;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
     const auto kernel = penalize_kernel<T, I, C>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_BYTES);
     if (e != cudaSuccess) return e;
-    kernel<<<(unsigned)blocks, THREADS, a.ids ? (size_t)chunks * CHUNK * sizeof(C) : 0, stream>>>(a, (int)pieces, chunks);
+    kernel<<<(unsigned)blocks, THREADS, (size_t)chunks * CHUNK * sizeof(C), stream>>>(a, (int)pieces, chunks);
     return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t penalize_t(const PenalizeArgs &a, cudaStream_t stream) {
+    if (!a.ids) {
+        constexpr int V = 16 / sizeof(T), EACH = 4, PIECE = THREADS * EACH * V;
+        const int64_t pieces = ((int64_t)a.v + V - 1 + PIECE - 1) / PIECE, blocks = pieces * a.b;
+        if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+        penalize_all_kernel<T, EACH><<<(unsigned)blocks, THREADS, 0, stream>>>(a, (int)pieces);
+        return cudaGetLastError();
+    }
     // (A counter of 16 bits counts to 32767.)
-    const bool small = !a.ids || a.t <= 0x7fff;
+    const bool small = a.t <= 0x7fff;
     if (a.ids_bytes == 8) return small ? run<T, int64_t, uint16_t>(a, stream) : run<T, int64_t, uint32_t>(a, stream);
     return small ? run<T, int32_t, uint16_t>(a, stream) : run<T, int32_t, uint32_t>(a, stream);
 }
