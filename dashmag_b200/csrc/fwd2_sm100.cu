@@ -152,8 +152,9 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     if constexpr (SPLIT) allow_beside();   // the merge
     const int b = blockIdx.z;
     // Tile t of the block: BT = 128 >> pack tokens from m_base + t BT on, of 1 << pack heads from h0 on.
-    const int pack = a.pack, bt = BM >> pack;
-    const int h0 = blockIdx.x << pack;
+    // (PREFIX: BM / heads sequences of a.heads heads, any number; the rows behind them are nobody's.)
+    const int pack = a.pack, bt = PREFIX ? BM / a.heads : BM >> pack;
+    const int h0 = PREFIX ? blockIdx.x * a.heads : blockIdx.x << pack;
     const int hk = h0 / (a.hq / a.hkv);
     const int m_base = qt * NT * bt;
     auto tile_row0 = [&](int t) { return m_base + t * bt; };
@@ -190,7 +191,7 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         // covers the rest of the setup.  (A block that turns out to have nothing to do waits for
         // them at the end: shared memory must not be written behind a block that has left.)
         const uint32_t qf = BAR(sh.bar.q_full);
-        mbar_expect_tx(qf, NT * Q_BYTES);
+        mbar_expect_tx(qf, PREFIX ? NT * HALVES * bt * a.heads * 128 : NT * Q_BYTES);
         for (int t = 0; t < NT; ++t) {
             const uint32_t dst = smem_u32(q_s + t * Q_BYTES);
 #pragma unroll
@@ -217,8 +218,8 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             if (lane == 0) sh.open[sw] = mine;
         }
         if constexpr (PREFIX) {
-            const int sequence = tile_row0(tile) + (r >> pack);
-            if (sequence < a.tq) prefix_bounds(a.reach, b, (int64_t)b * a.tq + sequence, lo, hi);
+            const int sequence = tile_row0(tile) + r / a.heads;
+            if (r < bt * a.heads && sequence < a.tq) prefix_bounds(a.reach, b, (int64_t)b * a.tq + sequence, lo, hi);
         } else {
             row_bounds_warp(a.mask, tile_row0(tile) + (r >> pack), a.tq, a.tk, lo, hi);
         }
@@ -394,8 +395,8 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         }
     } else if (!(solo && tile == 1)) {
         // ---------------- softmax of one tile, one row per thread ----------------
-        const int t = tile, h = h0 + (r & ((1 << pack) - 1));
-        const int row = tile_row0(t) + (r >> pack);
+        const int t = tile, h = h0 + (PREFIX ? r % a.heads : r & ((1 << pack) - 1));
+        const int row = PREFIX && r >= bt * a.heads ? a.tq : tile_row0(t) + (PREFIX ? r / a.heads : r >> pack);
         const uint32_t t_lane = tmem + (static_cast<uint32_t>(lane_base) << 16);
         const float2 sl2 = make_float2(a.scale_log2, a.scale_log2);
         float m_ref = -INFINITY, l = 0.f;
@@ -656,8 +657,8 @@ cudaError_t launch_fwd2_sm100(int dtype, const CUtensorMap &tq, const CUtensorMa
 
 cudaError_t launch_fwd2_prefix_sm100(int dtype, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Sm100FwdArgs &a,
                                      cudaStream_t stream) {
-    const int tokens = (NT * BM) >> a.pack;   // per block
-    dim3 grid(a.hq >> a.pack, (a.tq + tokens - 1) / tokens * a.splits, a.b);
+    const int sequences = NT * (BM / a.heads);   // per block
+    dim3 grid(a.hq / a.heads, (a.tq + sequences - 1) / sequences * a.splits, a.b);
     if (dtype == DASH_ATTN_BF16)
         return a.d <= 64 ? launch_fwd2_prefix_t<__nv_bfloat16, 64>(grid, tq, tk, tv, a, stream)
                          : launch_fwd2_prefix_t<__nv_bfloat16, 128>(grid, tq, tk, tv, a, stream);

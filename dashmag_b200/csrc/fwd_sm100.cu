@@ -114,13 +114,14 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // The tile: 128 >> pack tokens from m0 on, of 1 << pack heads from h0 on; row = token << pack | head.
     const int pack = a.pack;
-    const int h0 = blockIdx.x << pack;
+    const int heads = PREFIX ? a.heads : 1 << pack, bt = PREFIX ? BM / heads : BM >> pack;   // (PREFIX: any number of heads)
+    const int h0 = PREFIX ? blockIdx.x * heads : blockIdx.x << pack;
     const int split = SPLIT ? blockIdx.y % a.splits : 0;
     const int qt = SPLIT ? (gridDim.y - 1 - blockIdx.y) / a.splits : gridDim.y - 1 - blockIdx.y;  // later (longer, under causality) tiles first
     if constexpr (SPLIT) allow_beside();   // the merge
     const int b = blockIdx.z;
     const int hk = h0 / (a.hq / a.hkv);
-    const int m0 = qt * (BM >> pack);
+    const int m0 = qt * bt;
 
     const uint32_t q_full = smem_u32(&sh.bar.q_full), o_ready = smem_u32(&sh.bar.o_ready);
     auto BAR = [&](uint64_t (&arr)[2], int i) { return smem_u32(&arr[i]); };
@@ -156,8 +157,8 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     int lo = a.tk, hi = 0;
     if (warp >= 2 && warp < 6) {
         if constexpr (PREFIX) {
-            const int sequence = m0 + (r >> pack);
-            if (sequence < a.tq) prefix_bounds(a.reach, b, (int64_t)b * a.tq + sequence, lo, hi);
+            const int sequence = m0 + r / heads;
+            if (r < bt * heads && sequence < a.tq) prefix_bounds(a.reach, b, (int64_t)b * a.tq + sequence, lo, hi);
         } else {
             row_bounds_warp(a.mask, m0 + (r >> pack), a.tq, a.tk, lo, hi);
         }
@@ -184,7 +185,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     if (warp == 0) {
         // ---------------- TMA producer ----------------
         if (lane == 0 && n_tiles > 0) {
-            mbar_expect_tx(q_full, TILE_BYTES);
+            mbar_expect_tx(q_full, PREFIX ? PARTS * bt * heads * 128 : TILE_BYTES);
 #pragma unroll
             for (int part = 0; part < PARTS; ++part) tma_load_4d(smem_u32(q_s + part * HALF_BYTES), &tm_q, q_full, 64 * part, h0, m0, b);
             for (int j = 0; j < n_tiles && !failed; ++j) {
@@ -287,7 +288,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         }
     } else {
         // ---------------- softmax, one row per thread ----------------
-        const int row = m0 + (r >> pack), h = h0 + (r & ((1 << pack) - 1));
+        const int row = PREFIX && r >= bt * heads ? a.tq : m0 + (PREFIX ? r / heads : r >> pack), h = h0 + (PREFIX ? r % heads : r & ((1 << pack) - 1));
         const uint32_t t_lane = tmem + (static_cast<uint32_t>(lane_base) << 16);
         const bool padded = !PREFIX && a.mask.kind == 1;
         float m_ref = -INFINITY, l = 0.f;
@@ -498,8 +499,8 @@ cudaError_t launch_fwd_prefix_t(dim3 grid, const CUtensorMap &tq, const CUtensor
 
 cudaError_t launch_fwd_prefix_sm100(int dtype, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Sm100FwdArgs &a,
                                     cudaStream_t stream) {
-    const int tokens = BM >> a.pack;
-    dim3 grid(a.hq >> a.pack, (a.tq + tokens - 1) / tokens * a.splits, a.b);
+    const int sequences = BM / a.heads;
+    dim3 grid(a.hq / a.heads, (a.tq + sequences - 1) / sequences * a.splits, a.b);
     return dtype == DASH_ATTN_BF16 ? launch_fwd_prefix_t<__nv_bfloat16>(grid, tq, tk, tv, a, stream)
                                    : launch_fwd_prefix_t<__half>(grid, tq, tk, tv, a, stream);
 }

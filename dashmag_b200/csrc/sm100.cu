@@ -328,6 +328,20 @@ cudaError_t sm100_forward(const dash_attn_params *p, const TrainArgs &a, void *w
     return e;
 }
 
+// Heads of a group that share a tile of the prompts' part, any divisor: the one with the fewest tiles, and of those the largest (a tile's rows
+// beyond whole sequences are idle, and so are they where sequences are few: groups of six as pairs, 16 prompts of four sequences,
+// were three tiles of eight rows to a key-value head, and read its keys three times).
+static int prefix_heads(int group, int each) {
+    int best = 1;
+    int64_t least = -1;
+    for (int h = 1; h <= group && h <= 128; ++h) {
+        if (group % h != 0) continue;
+        const int64_t tiles = (each + 128 / h - 1) / (128 / h) * (int64_t)(group / h);
+        if (least < 0 || tiles <= least) { best = h; least = tiles; }
+    }
+    return best;
+}
+
 // The prompts' part of a decoding step over shared prompts: runs of keys a tile of rows is cut into.  Estimated in us, from forward_splits'
 // steps: a block's share of its sweep and what it costs however short that is, in waves; but the pass over the sequences' own
 // keys runs beside it, on the multiprocessors it leaves and then on all, so that what both cost of the GPU's time is a bound too; and the f32 rows
@@ -336,10 +350,10 @@ int sm100_prefix_splits(int dtype, float scale, int n, int each, int p, int hq, 
     // (Heads of a multiple of eight features: as 64, 128 or 256 with zeros behind them, which the copies bring.)
     if (dtype == DASH_ATTN_F32 || d % 8 != 0 || d > 256 || !(scale > 0.f) || !std::isfinite(scale)) return 0;
     const bool one = d > 128;
-    const int pack = pack_log2(hq / hkv, each);
-    const int64_t sequences = (one ? 128 : 256) >> pack, keys = one ? 128 : 64, sms = 148, tiles = (each + sequences - 1) / sequences;
-    if ((hq >> pack) > 65535 || n > 65535 || tiles > 65535) return 0;
-    const int64_t blocks = tiles * (hq >> pack) * n, l = (p + keys - 1) / keys;
+    const int heads = prefix_heads(hq / hkv, each);
+    const int64_t sequences = (one ? 1 : 2) * (128 / heads), keys = one ? 128 : 64, sms = 148, tiles = (each + sequences - 1) / sequences;
+    if (hq / heads > 65535 || n > 65535 || tiles > 65535) return 0;
+    const int64_t blocks = tiles * (hq / heads) * n, l = (p + keys - 1) / keys;
     const bool solo = !one && 2 * each <= sequences;
     const double step = one ? 1.8 : solo ? 0.6 : 0.95, fixed = one ? 5.4 : 5.7, own = own_bytes / 6.5e6;
     const double part = (double)n * each * hq * d * sizeof(float) / 2.3e6;
@@ -368,16 +382,16 @@ bool sm100_prefix_takes(const PrefixArgs &a) {
 }
 bool sm100_prefix(int dtype, const PrefixArgs &a, cudaStream_t stream, int *launches, cudaError_t *error) {
     CUtensorMap tq, tk, tv;
-    const int pack = pack_log2(a.hq / a.hkv, a.each);
+    const int heads = prefix_heads(a.hq / a.hkv, a.each);
     const int64_t qs[4] = {a.q_sb * a.each, a.q_sb, a.q_sh, a.q_sd}, ks[4] = {a.k.sb, a.k.st, a.k.sh, a.k.sd}, vs[4] = {a.v.sb, a.v.st, a.v.sh, a.v.sd};
-    if (!encode(&tq, dtype, a.q, a.n, a.each, a.hq, qs, 128, a.d, 1 << pack) || !encode(&tk, dtype, a.k.ptr, a.n, a.p, a.hkv, ks, 128, a.d) ||
+    if (!encode(&tq, dtype, a.q, a.n, a.each, a.hq, qs, 128, a.d, heads) || !encode(&tk, dtype, a.k.ptr, a.n, a.p, a.hkv, ks, 128, a.d) ||
         !encode(&tv, dtype, a.v.ptr, a.n, a.p, a.hkv, vs, 128, a.d))
         return false;
     Sm100FwdArgs f{};
     f.b = a.n; f.tq = a.each; f.tk = a.p; f.hq = a.hq; f.hkv = a.hkv; f.d = a.d;
     f.scale = a.scale;
     f.scale_log2 = a.scale * 1.4426950408889634f;
-    f.pack = pack;
+    f.heads = heads;
     f.splits = a.splits;
     f.part_o = a.part_o;
     f.part_lse = a.part_lse;

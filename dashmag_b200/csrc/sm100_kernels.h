@@ -22,6 +22,7 @@ struct Sm100FwdArgs {
     int splits;
     float *part_o;     // [splits][B,Tq,Hq,D]
     float *part_lse;   // [splits][B,Tq,Hq]
+    int heads;         // the prefix form: a tile is 128 / heads sequences of `heads` heads of one group, row = sequence * heads + head
     int beside;        // the prefix form: beside the launch in front of it, whose end is then this one's too
     PrefixReach reach; // the prefix form: which keys of its prompt each sequence sees (the mask is not looked at)
 };

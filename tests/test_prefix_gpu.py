@@ -77,6 +77,10 @@ DIMS = [
     (2, 3, 777, 33, 6, 2, 80),         # features that fill no tile
     (2, 5, 200, 70, 8, 2, 136),
     (3, 4, 150, 300, 4, 4, 24),
+    (16, 4, 200, 40, 24, 4, 64),       # groups of six: the rows of a tile that are nobody's
+    (2, 50, 150, 20, 20, 4, 128),      # of five
+    (1, 9, 300, 20, 14, 2, 256),       # of seven
+    (1, 3, 300, 20, 96, 2, 128),       # of forty-eight
     (3, 2, 63, 5, 3, 3, 51),           # on the CUDA cores whatever the dtype
     (1, 100, 200, 3, 10, 2, 32),
     (1, 1, 5000, 100, 32, 8, 128),     # one sequence, its prompt over the whole GPU
