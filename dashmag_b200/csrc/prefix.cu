@@ -28,7 +28,7 @@ namespace {
 // values of the same keys in shared memory as f32, scores and outputs in registers, two rows of four keys and of D / 16 features to a
 // thread, sixteen threads to a row.  The values are on their way to registers while the scores are made, the next keys while the outputs
 // are.  f32 products and sums throughout, bound by the FMA pipe and its operands from shared memory; with few rows by the trips to
-// memory (two prompts of 777 keys, three sequences each, 6 / 2 heads of 80 in f32: 41 us one element a load, waited for, now XX).
+// memory (two prompts of 777 keys, three sequences each, 6 / 2 heads of 80 in f32: 41 us one element a load, waited for, now 19 for all of the step).
 constexpr int ROWS = 32, KEYS = 64, THREADS = 256, MAX_D = 256;
 
 // Floats between rows of shared memory: whole 16-byte vectors, an odd number of them, so that eight rows' lie in banks of their own.
@@ -115,11 +115,31 @@ __global__ void __launch_bounds__(THREADS) prefix_generic_kernel(PrefixArgs a) {
         hi = warp_max_i(hi);
         if (threadIdx.x == 0) { span[0] = lo; span[1] = hi; }
     }
+    // The queries: eight threads a row, eight loads of each at once, asked for beside the lengths.
     // (Columns behind the features, up to a whole vector: zeros, in the keys too, which are written but for them.)
-#pragma unroll 4
-    for (int i = threadIdx.x; i < ROWS * 4 * d4; i += THREADS) {
-        const int r = i / (4 * d4), c = i - r * 4 * d4;
-        qs[r * pitch + c] = r0 + r < rows && c < a.d ? Num<T>::to_f32(static_cast<const T *>(a.q)[sequence(r0 + r) * a.q_sb + head(r0 + r) * a.q_sh + c * a.q_sd]) : 0.f;
+    {
+        struct alignas(VE > 1 ? 16 : sizeof(T)) Item { T e[VE]; };
+        const int qr = threadIdx.x / 8, per = a.d / VE;
+        const int64_t r = r0 + qr;
+        const T *from = static_cast<const T *>(a.q) + (r < rows ? sequence(r) * a.q_sb + head(r) * a.q_sh : 0);
+        float *to = qs + qr * pitch;
+        for (int i0 = threadIdx.x % 8; i0 < per; i0 += 64) {
+            Item x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (r >= rows || i0 + 8 * j >= per) continue;
+                if constexpr (VE > 1) *reinterpret_cast<uint4 *>(&x[j]) = *reinterpret_cast<const uint4 *>(from + (i0 + 8 * j) * VE);
+                else x[j].e[0] = from[(i0 + 8 * j) * a.q_sd];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (i0 + 8 * j >= per) continue;
+#pragma unroll
+                for (int e = 0; e < VE; ++e) to[(i0 + 8 * j) * VE + e] = r < rows ? Num<T>::to_f32(x[j].e[e]) : 0.f;
+            }
+        }
+        if (threadIdx.x % 8 == 0)
+            for (int c = a.d; c < 4 * d4; ++c) to[c] = 0.f;
     }
     if (a.d % 4 != 0)
         for (int i = threadIdx.x; i < KEYS * 4; i += THREADS)
@@ -186,7 +206,7 @@ __global__ void __launch_bounds__(THREADS) prefix_generic_kernel(PrefixArgs a) {
         if (k0 + KEYS < kmax) keys.ask(k0 + KEYS);
         const int there = min(KEYS, kmax - k0);
         const float *p0 = ps + 2 * ty * (KEYS + 4), *p1 = p0 + KEYS + 4;
-#pragma unroll 4
+#pragma unroll 8
         for (int k = 0; k < there; ++k) {
             const float w0 = p0[k], w1 = p1[k];
 #pragma unroll
@@ -243,7 +263,7 @@ __global__ void __launch_bounds__(THREADS) prefix_append_kernel(DecodeArgs a) {
 // parts' log-sum-exps and features at once, the first eight before it is known how many chunks the sequence's own keys make, and keeps
 // maximum, sum and outputs as the softmax does; the lanes' groups and the warps meet in order, so the bits repeat.
 // Bound by launch and latency, the parts being in L2: one trip to memory for most calls (one for the lengths, one for the log-sum-exps, one for the
-// parts: 2048 rows of 128 in five runs and up to eight chunks 9 us of a 45 us step, now XX).
+// parts: 32 prompts of sixteen answers, 8192 rows of 64, 56 us the step, now 51).
 constexpr int MERGE_THREADS = 128, MERGE_EACH = 8;
 
 template <typename T, int WARPS, int LANES, int J>
@@ -393,7 +413,7 @@ cudaError_t generic_t(const PrefixArgs &a, dim3 grid, cudaStream_t stream) {
     auto vectors = [&](const View4 &t) {
         return reinterpret_cast<uintptr_t>(t.ptr) % 16 == 0 && t.sd == 1 && t.sb % V == 0 && t.st % V == 0 && t.sh % V == 0;
     };
-    return a.d % V == 0 && vectors(a.k) && vectors(a.v) ? generic_v<T, V>(a, grid, stream) : generic_v<T, 1>(a, grid, stream);
+    return a.d % V == 0 && vectors(a.k) && vectors(a.v) && vectors(View4{a.q, 0, a.q_sb, a.q_sh, a.q_sd}) ? generic_v<T, V>(a, grid, stream) : generic_v<T, 1>(a, grid, stream);
 }
 
 template <typename T, int WARPS>
