@@ -829,7 +829,7 @@ int dash_attn_decode_shared(const dash_attn_decode_params *p, const dash_attn_pr
         b.reach = dash::PrefixReach{p->lengths, nullptr, p->lengths_elem_bytes, 0, p->s, 0, 0, append ? 1 : 0, own.left};
         sweep(b, s.own_tensor, s.own_generic);
     } else if (e == cudaSuccess && !refused && p->s > 0) {
-        e = dash::launch_decode_parts(p->dtype, own, true, true, stream, &launches);
+        e = dash::launch_decode_parts(p->dtype, own, stream, &launches);
     }
     if (refused) {
         g_probe[DASH_ATTN_PROBE_KERNEL_LAUNCHES] += launches;
@@ -847,6 +847,17 @@ int dash_attn_decode_shared(const dash_attn_decode_params *p, const dash_attn_pr
 // ------------------------------------------------------------------------------------------------
 // The rules on a step's logits
 // ------------------------------------------------------------------------------------------------
+// Whether out shares memory with the logits other than by being them: blocks would write what others still read.
+static bool rows_meet(const dash_sample_penalize_params *p, const void *logits, const void *out) {
+    const int64_t e = (int64_t)elem_bytes(p->dtype), row = p->v * e, hop = p->b > 1 ? p->out_stride * e : row;
+    const int64_t in_hop = p->b > 1 ? p->row_stride * e : row, to = (int64_t)reinterpret_cast<uintptr_t>(out) - (int64_t)reinterpret_cast<uintptr_t>(logits);
+    if (to == 0 && hop == in_hop) return false;
+    if (to >= (p->b - 1) * in_hop + row || -to >= (p->b - 1) * hop + row) return false;
+    if (hop != in_hop) return true;
+    const int64_t behind = ((to % hop) + hop) % hop;   // columns of one larger tensor: out's begin so far behind the logits'
+    return behind < row || hop - behind < row;
+}
+
 int dash_sample_penalize(const dash_sample_penalize_params *p, const void *logits, void *out, dash_attn_stream_t stream_) {
     const char *op = "penalize";
     g_error.clear();
@@ -872,6 +883,7 @@ int dash_sample_penalize(const dash_sample_penalize_params *p, const void *logit
     if (p->b == 0 || p->v == 0) return DASH_ATTN_OK;
     if (!logits || !out) return fail(DASH_ATTN_INVALID, "%s: a tensor pointer is null", op);
     if (p->b > 1 && p->out_stride < p->v) return fail(DASH_ATTN_INVALID, "%s: out's rows overlap", op);
+    if (rows_meet(p, logits, out)) return fail(DASH_ATTN_INVALID, "%s: out lies over the logits and is not them", op);
     dash::PenalizeArgs a{};
     a.logits = logits; a.out = out; a.b = p->b; a.v = p->v;
     a.stride = p->row_stride; a.out_stride = p->out_stride;

@@ -614,7 +614,7 @@ bool penalty_of(PyObject *rules, const char *name, const at::Tensor &z, bool his
     *all = nothing;
     if (PyFloat_Check(o.p) || PyLong_Check(o.p)) return float_of(o.p, all) && (history || *all == nothing);
     const at::Tensor *t = plain(o.p);
-    if (!t || t->dim() != 1 || t->size(0) != z.size(0) || t->scalar_type() != at::kFloat || !t->is_contiguous() || t->get_device() != z.get_device()) return false;
+    if (!history || !t || t->dim() != 1 || t->size(0) != z.size(0) || t->scalar_type() != at::kFloat || !t->is_contiguous() || t->get_device() != z.get_device()) return false;
     held.push_back(*t);
     *each = static_cast<const float *>(pointer(*t));
     return true;

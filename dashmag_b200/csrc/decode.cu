@@ -894,11 +894,8 @@ __global__ void __launch_bounds__(WARPS * 32) decode_split_mma_kernel(DecodeArgs
 
 // The same split for inputs the vector loads cannot take: one warp per (chunk, query head), a
 // lane owning the head dimensions `lane + 32 i`, keys in order.
-template <typename T, bool JOIN>
+template <typename T>
 __global__ void __launch_bounds__(DEC_WARPS * 32) decode_split_scalar_kernel(DecodeArgs a) {
-    if constexpr (JOIN) {
-        if (blockIdx.x == gridDim.x - 1) { end_beside(); return; }
-    }
     allow_beside();   // the merge
     const int lane = threadIdx.x & 31;
     const int b = blockIdx.y;
@@ -1243,7 +1240,7 @@ bool decode_fuses_rope(int dtype, const DecodeArgs &a, bool vector_ok) {
     return dtype != 0 && decode_uses_mma(2, a, vector_ok) && a.rope_dim % 16 == 0 && aligned(a.rope_cos) && aligned(a.rope_sin);
 }
 
-// The split pass; *merged: it left the outputs, and no parts.
+// The split pass; *merged: it left the outputs, and no parts.  (`beside`: with vectors only.)
 template <typename T>
 static cudaError_t split_t(const DecodeArgs &a, bool vector_ok, bool beside, cudaStream_t stream, bool *merged) {
     cudaError_t e;
@@ -1256,8 +1253,9 @@ static cudaError_t split_t(const DecodeArgs &a, bool vector_ok, bool beside, cud
     else if (vector_ok && a.d == 256) e = split_vec<T, 256>(a, beside, stream);
     else {
         const long long units = (long long)a.splits * a.hq;
-        dim3 grid((unsigned)((units + DEC_WARPS - 1) / DEC_WARPS + beside), a.b);
-        e = launch_beside(beside ? decode_split_scalar_kernel<T, true> : decode_split_scalar_kernel<T, false>, grid, DEC_WARPS * 32, 0, stream, beside, a);
+        dim3 grid((unsigned)((units + DEC_WARPS - 1) / DEC_WARPS), a.b);
+        decode_split_scalar_kernel<T><<<grid, DEC_WARPS * 32, 0, stream>>>(a);
+        e = cudaGetLastError();
     }
     return e;
 }
@@ -1295,12 +1293,12 @@ cudaError_t launch_decode(int dtype, const DecodeArgs &a, bool vector_ok, cudaSt
     }
 }
 
-cudaError_t launch_decode_parts(int dtype, const DecodeArgs &a, bool vector_ok, bool beside, cudaStream_t stream, int *launches) {
+cudaError_t launch_decode_parts(int dtype, const DecodeArgs &a, cudaStream_t stream, int *launches) {
     *launches += 1;
     switch (dtype) {
-        case 0: return split_t<float>(a, vector_ok, beside, stream, nullptr);
-        case 1: return split_t<__nv_bfloat16>(a, vector_ok, beside, stream, nullptr);
-        default: return split_t<__half>(a, vector_ok, beside, stream, nullptr);
+        case 0: return split_t<float>(a, true, true, stream, nullptr);
+        case 1: return split_t<__nv_bfloat16>(a, true, true, stream, nullptr);
+        default: return split_t<__half>(a, true, true, stream, nullptr);
     }
 }
 

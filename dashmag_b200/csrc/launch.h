@@ -17,9 +17,9 @@ cudaError_t launch_generic_delta(int dtype, const TrainArgs &a, cudaStream_t str
 bool decode_fuses_rope(int dtype, const DecodeArgs &a, bool vector_ok);
 long long decode_fixed_chunk();
 cudaError_t launch_decode(int dtype, const DecodeArgs &a, bool vector_ok, cudaStream_t stream, int *launches);
-// The split pass alone, in chunks: its parts are merged with others (prefix.cu).  `beside`: beside the launch in front of it, whose end is then
-// this pass's too.
-cudaError_t launch_decode_parts(int dtype, const DecodeArgs &a, bool vector_ok, bool beside, cudaStream_t stream, int *launches);
+// The split pass alone over a cache read by vectors, in chunks, whose parts are merged with others (prefix.cu): beside the launch in front of it,
+// whose end is then this pass's too.
+cudaError_t launch_decode_parts(int dtype, const DecodeArgs &a, cudaStream_t stream, int *launches);
 // The library's own decode scratch: its size in floats, and its address on the current device.
 size_t decode_static_capacity_floats();
 cudaError_t decode_static_scratch(float **out);

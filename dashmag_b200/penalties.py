@@ -39,8 +39,8 @@ class Penalties:
 
 
 def penalize(logits: torch.Tensor, penalties: Penalties, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``logits [B, V]`` (f32, bf16 or f16) under ``penalties``, f32 arithmetic rounded once; into ``out`` (which may be the logits) where
-    given."""
+    """``logits [B, V]`` (f32, bf16 or f16) under ``penalties``, f32 arithmetic rounded once; into ``out`` (which may be the logits, but
+    not other memory of theirs) where given.  Not differentiable (as ``sample`` itself)."""
     if out is None:
         done = _lib.binding().penalize(logits, penalties)
         if done is not None:
@@ -83,6 +83,8 @@ def penalize(logits: torch.Tensor, penalties: Penalties, out: Optional[torch.Ten
         if isinstance(x, torch.Tensor):
             if tuple(x.shape) != (b,) or x.dtype != torch.float32:
                 raise AttentionError(f"{op}: the {name} penalty is a number or f32 [B] = [{b}], got {x.dtype} {list(x.shape)}")
+            if tokens is None:
+                raise AttentionError(f"{op}: a {name} penalty needs the tokens")
             keep.append(x.contiguous())
             setattr(p, name, _ptr(keep[-1]))
             x = nothing

@@ -320,7 +320,7 @@ typedef struct dash_sample_penalize_params {
     int64_t allowed_stride;       /* words between rows; 0: one row for all */
 } dash_sample_penalize_params;
 
-/* out may be the logits themselves, with the same row stride. */
+/* out may be the logits themselves, with the same row stride; other memory of theirs is refused. */
 int dash_sample_penalize(const dash_sample_penalize_params *p, const void *logits, void *out, dash_attn_stream_t stream);
 
 /*
@@ -386,7 +386,7 @@ int dash_attn_kernels_take(const dash_attn_params *p, const void *q, const void 
                            int backward);
 
 /*
- * Every wait inside the tensor-core kernels is bounded; one that runs out raises a sticky word on
+ * Every wait inside the tensor-core kernels, and the norm's for its bulk copies, is bounded; one that runs out raises a sticky word on
  * the device instead of hanging, and later blocks and launches of those kernels then do nothing.
  * This reads that word (0 = healthy) and, with `clear` non-zero, resets it.  It synchronises with
  * the device, so it is for tests and for error paths, not for the hot loop.  Returns a negative

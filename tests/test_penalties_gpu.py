@@ -196,3 +196,17 @@ def test_nothing_to_do():
     assert penalize(torch.zeros((0, 10), device=DEV), Penalties()).shape == (0, 10)
     assert penalize(torch.zeros((4, 0), device=DEV), Penalties()).shape == (4, 0)
     assert _lib.probe("kernel_launches") == before
+
+
+@pytest.mark.parametrize("dtype", list(TORCH))
+def test_out_in_other_columns_of_the_logits_tensor(dtype):
+    """Logits and result are columns of one larger tensor, side by side, without a token in common."""
+    b, v = 4, 333
+    logits, p = case(b, v, 50, dtype, 11, "rows", True)
+    both = torch.zeros((b, 2 * v + 3), device=DEV, dtype=TORCH[dtype])
+    for left in (True, False):
+        both.zero_()
+        source, out = (both[:, :v], both[:, v + 3:]) if left else (both[:, v + 3:], both[:, :v])
+        source.copy_(logits)
+        penalize(source, p, out=out)
+        assert torch.equal(out, penalize(logits, p)) and torch.equal(source, logits) and not bool(both[:, v:v + 3].any())

@@ -190,3 +190,24 @@ def test_structs_are_the_headers(tmp_path):
     subprocess.run(["gcc", str(source), "-o", str(tmp_path / "sizes")], check=True)
     got = list(map(int, subprocess.run([str(tmp_path / "sizes")], capture_output=True, text=True, check=True).stdout.split()))
     assert got == [x for s in names.values() for x in (ctypes.sizeof(s), *(getattr(s, f[0]).offset for f in s._fields_))]
+
+
+def test_rules_refuse_memory_they_would_read_after_writing_it():
+    lib = _lib.lib()
+    at = 1 << 20
+
+    def rc(out, row=100, out_row=100, b=3, v=40):
+        p = _lib.PenalizeParams(dtype=2, b=b, v=v, row_stride=row, out_stride=out_row, repetition_all=1.0)
+        return lib.dash_sample_penalize(ctypes.byref(p), at, out, None)
+
+    for out, kw in ((at + 2, {}), (at - 2, {}), (at + 2 * 100 + 2 * 39, {}), (at + 2 * 200 + 2 * 39, {}), (at - 2 * 200 - 2 * 39, {}), (at + 2 * 61, {}),
+                    (at, dict(out_row=101)), (at, dict(row=0)), (at + 2 * 239, dict(out_row=50)), (at - 2 * 139, dict(out_row=50)),
+                    (at + 2 * 39, dict(b=1)), (at - 2 * 39, dict(b=1))):
+        assert rc(out, **kw) == _lib.INVALID and "not them" in _lib.last_error(), (out - at, kw)
+
+
+def test_rules_want_the_tokens_for_a_tensor_of_penalties():
+    z = torch.zeros((2, 40))
+    for name in ("repetition", "frequency", "presence"):
+        with pytest.raises(AttentionError, match="needs the tokens"):
+            penalize(z, Penalties(**{name: torch.ones(2)}))
