@@ -42,8 +42,8 @@ Over over_of(int64_t d) {   // (1 <= d < 2^31)
 struct RingPlan {
     int heads, units;    // of a token; units of them to a token
     int tokens;          // of a stage
+    int slots;           // of them that the lanes of a warp take at once, a power of two
     int stage;           // bytes
-    Over over_heads;
 };
 
 // n / d for 0 <= n < 2^31 and d >= 1 by a multiplication (Granlund and Montgomery: m = floor(2^32 (2^l - d) / d) + 1, l = ceil(log2 d)).
@@ -385,6 +385,7 @@ __global__ void __launch_bounds__(Ring<BACK>::WARPS * 32, Ring<BACK>::BLOCKS) qk
     const int64_t tokens = set < sets && *reinterpret_cast<volatile unsigned int *>(&g_qk_norm_status) == 0 ? a.b * a.t : 0;
     const int64_t first = (int64_t)set * each, step = (int64_t)sets * each;
     const Place<V, LPH> at(a, lane);
+    const int slots = plan.slots, beside = NG / slots, slot = lane / LPH / beside, part = lane / LPH % beside;   // tokens at once, heads of each
     const Weights<TW, V, LPH> w(t.w, at);
     const float inv_d = 1.f / a.d;
     float2 d1[V / 2], d2[V / 2];
@@ -433,63 +434,62 @@ __global__ void __launch_bounds__(Ring<BACK>::WARPS * 32, Ring<BACK>::BLOCKS) qk
             const T *xs = reinterpret_cast<const T *>(stage + xs_at), *ys = reinterpret_cast<const T *>(stage + ys_at);
             T *out = static_cast<T *>(t.out) + (n * t.heads + h0) * a.d;
             const unsigned kinds = what >> (2 * s) & 3u;
-            unsigned kind = __shfl_sync(0xffffffffu, kinds, 0);
-            Factors<T, TW, V, LPH, BACK> f;
-            if (!many) f.set(reinterpret_cast<const T *>(stage), a.dim, at, w, kind);
-            const int rows = (int)min((int64_t)each, tokens - n) * heads;
+            const int there = (int)min((int64_t)each, tokens - n);
+            // The lanes of a head take heads of one token in turn, so that its factors, which cost more than a head, are made once for them.
+            for (int token0 = 0; token0 < there; token0 += slots) {
+                const int token = min(token0 + slot, there - 1);
+                const unsigned kind = __shfl_sync(0xffffffffu, kinds, token);
+                Factors<T, TW, V, LPH, BACK> f;
+                f.set(reinterpret_cast<const T *>(stage + token * 2 * row_size), a.dim, at, w, kind);
 #pragma unroll 2
-            for (int r0 = 0; r0 < rows; r0 += NG) {
-                const int row = r0 + lane / LPH;   // the head, of the stage's all
-                const bool live = at.live && row < rows;
-                if (many) {
-                    const int token = min((int)over((uint32_t)row, plan.over_heads), each - 1);
-                    kind = __shfl_sync(0xffffffffu, kinds, token);
-                    f.set(reinterpret_cast<const T *>(stage + token * 2 * row_size), a.dim, at, w, kind);
-                }
-                float2 u1[V / 2], u2[V / 2], g1[V / 2], g2[V / 2], square = both(0.f), along = both(0.f);
-                Vec<T, V> y1, y2;
-                if (live) {
-                    const Vec<T, V> x1 = load<T, V>(xs + row * a.d + at.c1), x2 = load<T, V>(xs + row * a.d + at.c2);
-                    if constexpr (BACK) {
-                        y1 = load<T, V>(ys + row * a.d + at.c1);
-                        y2 = load<T, V>(ys + row * a.d + at.c2);
-                    } else {
-                        y1 = x1;
-                        y2 = x2;
-                    }
-#pragma unroll
-                    for (int i = 0; i < V / 2; ++i) {
-                        u1[i] = pair<V>(x1, i);
-                        u2[i] = pair<V>(x2, i);
-                        square = ptx::fma2(u1[i], u1[i], ptx::fma2(u2[i], u2[i], square));
+                for (int r0 = 0; r0 < heads; r0 += beside) {
+                    const int row = token * heads + r0 + part;   // the head, of the stage's all
+                    const bool live = at.live && r0 + part < heads && token0 + slot < there;
+                    float2 u1[V / 2], u2[V / 2], g1[V / 2], g2[V / 2], square = both(0.f), along = both(0.f);
+                    Vec<T, V> y1, y2;
+                    if (live) {
+                        const Vec<T, V> x1 = load<T, V>(xs + row * a.d + at.c1), x2 = load<T, V>(xs + row * a.d + at.c2);
                         if constexpr (BACK) {
-                            const float2 v1 = pair<V>(y1, i), v2 = pair<V>(y2, i);
-                            g1[i] = ptx::fma2(v1, f.k1[i], ptx::mul2(v2, f.z2[i]));
-                            g2[i] = ptx::fma2(v2, f.k2[i], ptx::mul2(v1, f.z1[i]));
-                            along = ptx::fma2(ptx::mul2(g1[i], pair<V>(w.w1, i)), u1[i], ptx::fma2(ptx::mul2(g2[i], pair<V>(w.w2, i)), u2[i], along));
-                        }
-                    }
-                }
-                const float r = rsqrtf(fmaf(head_sum<LPH>(square.x + square.y), inv_d, a.eps));
-                const float back = BACK ? -head_sum<LPH>(along.x + along.y) * inv_d * r : 0.f;
-                if (!live) continue;
-                if (kind != 2) {   // (a token of no sequence passes unchanged, and so does its gradient)
-#pragma unroll
-                    for (int i = 0; i < V / 2; ++i) {
-                        if constexpr (BACK) {
-                            const float2 n1 = ptx::mul2(u1[i], both(r)), n2 = ptx::mul2(u2[i], both(r));
-                            put<V>(y1, i, ptx::mul2(ptx::fma2(n1, both(back), ptx::mul2(g1[i], pair<V>(w.w1, i))), both(r)));
-                            put<V>(y2, i, ptx::mul2(ptx::fma2(n2, both(back), ptx::mul2(g2[i], pair<V>(w.w2, i))), both(r)));
-                            d1[i] = ptx::fma2(g1[i], n1, d1[i]);
-                            d2[i] = ptx::fma2(g2[i], n2, d2[i]);
+                            y1 = load<T, V>(ys + row * a.d + at.c1);
+                            y2 = load<T, V>(ys + row * a.d + at.c2);
                         } else {
-                            put<V>(y1, i, ptx::mul2(ptx::fma2(u1[i], f.k1[i], ptx::mul2(u2[i], f.z1[i])), both(r)));
-                            put<V>(y2, i, ptx::mul2(ptx::fma2(u2[i], f.k2[i], ptx::mul2(u1[i], f.z2[i])), both(r)));
+                            y1 = x1;
+                            y2 = x2;
+                        }
+#pragma unroll
+                        for (int i = 0; i < V / 2; ++i) {
+                            u1[i] = pair<V>(x1, i);
+                            u2[i] = pair<V>(x2, i);
+                            square = ptx::fma2(u1[i], u1[i], ptx::fma2(u2[i], u2[i], square));
+                            if constexpr (BACK) {
+                                const float2 v1 = pair<V>(y1, i), v2 = pair<V>(y2, i);
+                                g1[i] = ptx::fma2(v1, f.k1[i], ptx::mul2(v2, f.z2[i]));
+                                g2[i] = ptx::fma2(v2, f.k2[i], ptx::mul2(v1, f.z1[i]));
+                                along = ptx::fma2(ptx::mul2(g1[i], pair<V>(w.w1, i)), u1[i], ptx::fma2(ptx::mul2(g2[i], pair<V>(w.w2, i)), u2[i], along));
+                            }
                         }
                     }
+                    const float r = rsqrtf(fmaf(head_sum<LPH>(square.x + square.y), inv_d, a.eps));
+                    const float back = BACK ? -head_sum<LPH>(along.x + along.y) * inv_d * r : 0.f;
+                    if (!live) continue;
+                    if (kind != 2) {   // (a token of no sequence passes unchanged, and so does its gradient)
+#pragma unroll
+                        for (int i = 0; i < V / 2; ++i) {
+                            if constexpr (BACK) {
+                                const float2 n1 = ptx::mul2(u1[i], both(r)), n2 = ptx::mul2(u2[i], both(r));
+                                put<V>(y1, i, ptx::mul2(ptx::fma2(n1, both(back), ptx::mul2(g1[i], pair<V>(w.w1, i))), both(r)));
+                                put<V>(y2, i, ptx::mul2(ptx::fma2(n2, both(back), ptx::mul2(g2[i], pair<V>(w.w2, i))), both(r)));
+                                d1[i] = ptx::fma2(g1[i], n1, d1[i]);
+                                d2[i] = ptx::fma2(g2[i], n2, d2[i]);
+                            } else {
+                                put<V>(y1, i, ptx::mul2(ptx::fma2(u1[i], f.k1[i], ptx::mul2(u2[i], f.z1[i])), both(r)));
+                                put<V>(y2, i, ptx::mul2(ptx::fma2(u2[i], f.k2[i], ptx::mul2(u1[i], f.z2[i])), both(r)));
+                            }
+                        }
+                    }
+                    store<T, V>(out + row * a.d + at.c1, y1);
+                    store<T, V>(out + row * a.d + at.c2, y2);
                 }
-                store<T, V>(out + row * a.d + at.c1, y1);
-                store<T, V>(out + row * a.d + at.c2, y2);
             }
             s ^= 1;
         }
@@ -686,9 +686,9 @@ Plan plan_of(int dtype, const NormArgs &a, bool back) {
     const int64_t tokens = a.b * a.t;
     const int hg = back ? Ring<true>::HG : Ring<false>::HG, nw = back ? Ring<true>::WARPS : Ring<false>::WARPS;
     const int room = 148 * (back ? Ring<true>::BLOCKS : Ring<false>::BLOCKS);
-    // Warps that the tensors have work for, and what it costs, in loads of `ng` heads: a stage costs about as much as one and a half for its
-    // waiting and its factors, and where it is of several tokens their factors with every load (16384 tokens of 32 / 8 heads of 128, these
-    // counted like the others | as here: 71.6 | 63.7 us, backward 108 | 98: the blocks of one tensor waited for the other's).
+    // Warps that the tensors have work for, and what it costs, in loads of `ng` heads: a stage about as much as one and a half for its waiting,
+    // and where it is of several tokens, each turn of them one for their factors, and forward their loads more than half as much again.  (16384
+    // tokens, loads counted alike | as here, us: 32 / 8 heads of 128 71.0 | 66.1, 8 / 1 of 256 41.7 | 32.5: the blocks of one tensor waited for the other's.)
     int64_t want_q, want_k;
     double cost_q, cost_k;
     auto ring = [&](RingPlan &r, const NormTensor &t, int64_t &want, double &cost) {
@@ -697,19 +697,20 @@ Plan plan_of(int dtype, const NormArgs &a, bool back) {
         while (r.heads > ng && stage_bytes(back, r.heads, 1, a.d, a.dim, eb) > STAGE_MOST) r.heads -= ng;
         r.units = r.heads ? (t.heads + r.heads - 1) / r.heads : 0;
         r.tokens = r.heads ? std::max(1, std::min(32, ng * hg / r.heads)) : 1;
-        if (tokens < (int64_t)r.tokens * room * nw / 2) r.tokens = 1;   // (few tokens: rather more warps)
+        r.tokens = (int)std::min<int64_t>(r.tokens, std::max<int64_t>(1, tokens / (room * nw / 2)));   // (few tokens: rather more warps)
         while (r.tokens > 1 && stage_bytes(back, r.heads * r.tokens, r.tokens, a.d, a.dim, eb) > STAGE_MOST) --r.tokens;
         r.stage = stage_bytes(back, r.heads * r.tokens, r.tokens, a.d, a.dim, eb);
-        if (r.heads) r.over_heads = over_of(r.heads);
+        for (r.slots = 1; 2 * r.slots <= std::min(ng, r.tokens);) r.slots *= 2;
         want = ((tokens + r.tokens - 1) / r.tokens * r.units + nw - 1) / nw;
-        cost = r.units * ((double)((r.heads * r.tokens + ng - 1) / ng) * (r.tokens == 1 ? 1.0 : back ? 1.4 : 2.2) + 1.5) / r.tokens;
+        const int turns = (r.tokens + r.slots - 1) / r.slots, beside = ng / r.slots;
+        cost = r.units * (turns * ((r.heads + beside - 1) / beside * (r.tokens == 1 || back ? 1. : 1.6) + (r.tokens == 1 ? 0. : 1.)) + 1.5) / r.tokens;
     };
     ring(p.ring_q, a.q, want_q, cost_q);
     ring(p.ring_k, a.k, want_k, cost_k);
-    // The ring for the gradient, and forward in 16 bits where its warps get two stages each or more: one stage alone is waited for (us, ring |
-    // a warp for every token: bf16, 32 / 8 heads of 128, 4096 tokens 18.4 | 23.4, 16384 64 | 92, 1024 6.8 | 6.8; 16 / 4 of 64, 4096 11.9 | 8.6,
-    // 16384 24 | 33).  In f32 a byte has half the instructions, and loads into registers keep up with HBM: 8192 tokens 69 | 58.
-    p.way = !vec ? ELEMENTS : back || (eb == 2 && want_q + want_k >= 2 * room) ? RING : HEADS;
+    // The ring for the gradient, and forward in 16 bits where its warps get one and a half stages each or more: one stage alone is waited for (us, ring |
+    // a warp for every token: bf16, 32 / 8 heads of 128, 1000 tokens 8.4 | 6.7, 16384 64 | 92; 16 / 4 of 128, 2500 8.9 | 8.4, 5000 14.0 | 16.5;
+    // 8 / 1 of 64, 2500 6.5 | 5.9, 16384 15.7 | 25.9).  In f32 a byte has half the instructions, and loads into registers keep up with HBM: 8192 tokens 69 | 58.
+    p.way = !vec ? ELEMENTS : back || (eb == 2 && 2 * (want_q + want_k) >= 3 * room) ? RING : HEADS;
     if (p.way == HEADS) {
         p.units_q = (a.q.heads + ng * HEADS_EACH - 1) / (ng * HEADS_EACH);
         p.units_k = (a.k.heads + ng * HEADS_EACH - 1) / (ng * HEADS_EACH);
