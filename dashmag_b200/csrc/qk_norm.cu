@@ -121,17 +121,19 @@ __device__ __forceinline__ int64_t table_row_warp(const NormArgs &a, int64_t n, 
     return pos >= 0 && pos < a.len ? pos : -1;
 }
 
-// V elements of T as they lie in memory, 16 bytes (weights in f32 beside 16-bit tensors: 32), and as pairs of f32, two to a
-// packed instruction.
-template <typename T, int V> struct alignas(16) Vec { T e[V]; };
+// V elements of T as they lie in memory, 16 bytes or 8 (weights in f32 beside 16-bit tensors: twice that), and as pairs of f32, two
+// to a packed instruction.
+template <typename T, int V> struct alignas(sizeof(T) * V < 16 ? 8 : 16) Vec { T e[V]; };
 template <typename T, int V> __device__ __forceinline__ Vec<T, V> load(const T *p) {
     Vec<T, V> v;
+    if constexpr (sizeof(v) == 8) *reinterpret_cast<uint2 *>(&v) = *reinterpret_cast<const uint2 *>(p);
 #pragma unroll
     for (int i = 0; i < (int)sizeof(v) / 16; ++i) reinterpret_cast<uint4 *>(&v)[i] = reinterpret_cast<const uint4 *>(p)[i];
     return v;
 }
 template <typename T, int V> __device__ __forceinline__ void store(T *p, const Vec<T, V> &v) {
-    *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(&v);
+    if constexpr (sizeof(v) == 8) *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(&v);
+    else *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(&v);
 }
 template <int V> __device__ __forceinline__ float2 pair(const Vec<float, V> &v, int i) { return make_float2(v.e[2 * i], v.e[2 * i + 1]); }
 template <int V> __device__ __forceinline__ float2 pair(const Vec<__nv_bfloat16, V> &v, int i) {
@@ -662,7 +664,7 @@ __global__ void __launch_bounds__(THREADS) qk_norm_sum_kernel(NormArgs a, int bl
 enum Way { ELEMENTS, HEADS, RING };
 struct Plan {
     Way way;
-    int lph;                 // lanes of a head
+    int columns, lph;        // of a lane, twice; lanes of a head
     int units_q, units_k;    // HEADS: warps of a token
     RingPlan ring_q, ring_k;
     int blocks_q, blocks;    // the ring's and the element kernels' blocks: the queries', and all
@@ -679,8 +681,12 @@ Plan plan_of(int dtype, const NormArgs &a, bool back) {
                                 (!back || (aligned(t.g) && t.gb % v == 0 && t.gt % v == 0 && t.gh % v == 0)));
     };
     Plan p{};
-    const bool vec = a.dim % (2 * v) == 0 && a.d % (2 * v) == 0 && aligned(a.cos) && aligned(a.sin) && vectors(a.q) && vectors(a.k);
-    const int items = a.d / (2 * v);
+    // A lane's columns are 16 bytes where the halves that are paired are whole vectors, else (40 rotated of 80 in 16 bits) 8; the rows and the heads
+    // are whole vectors in any case, for the copies.  (16384 tokens of 16 / 4 such heads, element by element | so: 184 | 45 us, backward 411 | 69.)
+    auto whole = [&](int columns) { return a.dim % (2 * columns) == 0 && a.d % (2 * columns) == 0; };
+    p.columns = eb == 2 && !whole(v) ? v / 2 : v;
+    const bool vec = whole(p.columns) && aligned(a.cos) && aligned(a.sin) && vectors(a.q) && vectors(a.k);
+    const int items = a.d / (2 * p.columns);
     p.lph = items <= 4 ? 4 : items <= 8 ? 8 : items <= 16 ? 16 : 32;
     const int ng = 32 / p.lph;
     const int64_t tokens = a.b * a.t;
@@ -753,6 +759,16 @@ cudaError_t run_vec(const NormArgs &a, const Plan &p, bool back, cudaStream_t st
     return cudaGetLastError();
 }
 
+template <typename T, typename TW, int V>
+cudaError_t run_columns(const NormArgs &a, const Plan &p, bool back, cudaStream_t stream) {
+    switch (p.lph) {
+        case 4: return run_vec<T, TW, V, 4>(a, p, back, stream);
+        case 8: return run_vec<T, TW, V, 8>(a, p, back, stream);
+        case 16: return run_vec<T, TW, V, 16>(a, p, back, stream);
+        default: return run_vec<T, TW, V, 32>(a, p, back, stream);
+    }
+}
+
 template <typename T, typename TW>
 cudaError_t run_t(const NormArgs &a, const Plan &p, bool back, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
@@ -761,12 +777,9 @@ cudaError_t run_t(const NormArgs &a, const Plan &p, bool back, cudaStream_t stre
         else qk_norm_elements_kernel<T, false><<<p.blocks, THREADS, 0, stream>>>(a, p.blocks_q);
         return cudaGetLastError();
     }
-    switch (p.lph) {
-        case 4: return run_vec<T, TW, V, 4>(a, p, back, stream);
-        case 8: return run_vec<T, TW, V, 8>(a, p, back, stream);
-        case 16: return run_vec<T, TW, V, 16>(a, p, back, stream);
-        default: return run_vec<T, TW, V, 32>(a, p, back, stream);
-    }
+    if constexpr (sizeof(T) == 2)
+        if (p.columns < V) return run_columns<T, TW, V / 2>(a, p, back, stream);
+    return run_columns<T, TW, V>(a, p, back, stream);
 }
 
 cudaError_t run(int dtype, const NormArgs &a, const Plan &p, bool back, cudaStream_t stream) {

@@ -17,7 +17,7 @@ DEV = "cuda:0"
 TORCH = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 U = 2.0 ** -24
 # (features rotated, head dimension): whole heads, parts, a lane's columns that fill no warp, shapes too narrow or too ragged for vectors
-SHAPES = [(128, 128), (64, 128), (64, 64), (256, 256), (48, 96), (80, 80), (16, 16), (2, 2), (6, 17), (100, 250)]
+SHAPES = [(128, 128), (64, 128), (64, 64), (256, 256), (48, 96), (80, 80), (16, 16), (2, 2), (6, 17), (100, 250), (40, 80), (24, 72), (8, 8), (24, 256), (8, 200)]
 
 
 def smallest(dtype):
@@ -232,7 +232,7 @@ def test_in_place_through_the_c_abi(tokens, d):
 
 
 @pytest.mark.parametrize("dtype", list(TORCH))
-@pytest.mark.parametrize("hq,hkv,d,dim", [(32, 8, 128, 128), (16, 4, 64, 64), (8, 1, 64, 32), (5, 3, 96, 96), (70, 2, 32, 32), (12, 12, 256, 128)])
+@pytest.mark.parametrize("hq,hkv,d,dim", [(32, 8, 128, 128), (16, 4, 64, 64), (8, 1, 64, 32), (5, 3, 96, 96), (70, 2, 32, 32), (12, 12, 256, 128), (16, 4, 80, 40), (3, 1, 40, 24), (9, 2, 248, 8)])
 def test_many_tokens(hq, hkv, d, dim, dtype):
     """Long enough that every warp takes tokens one after another, several at a time where their heads are few, in sequences that end anywhere."""
     t = TORCH[dtype]
