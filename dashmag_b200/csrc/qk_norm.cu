@@ -713,10 +713,15 @@ Plan plan_of(int dtype, const NormArgs &a, bool back) {
     };
     ring(p.ring_q, a.q, want_q, cost_q);
     ring(p.ring_k, a.k, want_k, cost_k);
-    // The ring for the gradient, and forward in 16 bits where its warps get one and a half stages each or more: one stage alone is waited for (us, ring |
+    // The ring for the gradient, and forward in 16 bits where its warps get one and a half stages each or more: one alone is waited for (us, ring |
     // a warp for every token: bf16, 32 / 8 heads of 128, 1000 tokens 8.4 | 6.7, 16384 64 | 92; 16 / 4 of 128, 2500 8.9 | 8.4, 5000 14.0 | 16.5;
-    // 8 / 1 of 64, 2500 6.5 | 5.9, 16384 15.7 | 25.9).  In f32 a byte has half the instructions, and loads into registers keep up with HBM: 8192 tokens 69 | 58.
-    p.way = !vec ? ELEMENTS : back || (eb == 2 && 2 * (want_q + want_k) >= 3 * room) ? RING : HEADS;
+    // 8 / 1 of 64, 2500 6.5 | 5.9, 16384 15.7 | 25.9).  In f32 a byte has
+    // half the instructions, and loads into registers keep up with HBM (16384 tokens of 32 / 8 heads of 128 130 | 118) unless heads leave lanes
+    // idle and tokens are many (five stages a warp: 16 / 16 of 80, 5000 24.6 | 26.4, 16384 64.8 | 81.5; 32 / 8 of 96, 16384 85.6 | 108; below,
+    // 16 / 4 of 80, 5000 19.4 | 16.6).
+    const int64_t want = want_q + want_k;
+    const bool staged = eb == 2 ? 2 * want >= 3 * room : items < p.lph && want >= 5 * room;
+    p.way = !vec ? ELEMENTS : back || staged ? RING : HEADS;
     if (p.way == HEADS) {
         p.units_q = (a.q.heads + ng * HEADS_EACH - 1) / (ng * HEADS_EACH);
         p.units_k = (a.k.heads + ng * HEADS_EACH - 1) / (ng * HEADS_EACH);
