@@ -259,14 +259,14 @@ __global__ void __launch_bounds__(THREADS) prefix_append_kernel(DecodeArgs a) {
 // ---------------------------------------------------------------------------------------------
 // The merge
 // ---------------------------------------------------------------------------------------------
-// WARPS warps a row; LANES lanes a part (16 where a head is at most 64 features, else 32), four features or J times four each.  A lane asks for eight
-// parts' log-sum-exps and features at once, the first eight before it is known how many chunks the sequence's own keys make, and keeps
+// WARPS warps a row; LANES lanes a part (16 where a head is at most 64 features, else 32), four features or J times four each.  A lane asks for EACH
+// parts' log-sum-exps and features at once, the first of them before it is known how many chunks the sequence's own keys make, and keeps
 // maximum, sum and outputs as the softmax does; the lanes' groups and the warps meet in order, so the bits repeat.
 // Bound by launch and latency, the parts being in L2: one trip to memory for most calls (one for the lengths, one for the log-sum-exps, one for the
 // parts: 32 prompts of sixteen answers, 8192 rows of 64, 56 us the step, now 51).
-constexpr int MERGE_THREADS = 128, MERGE_EACH = 8;
+constexpr int MERGE_THREADS = 128;
 
-template <typename T, int WARPS, int LANES, int J>
+template <typename T, int WARPS, int EACH, int LANES, int J>
 __global__ void __launch_bounds__(MERGE_THREADS) prefix_merge_kernel(PrefixMergeArgs a) {
     constexpr int AT_ONCE = MERGE_THREADS / 32 / WARPS, SUBS = 32 / LANES, STEP = WARPS * SUBS;   // rows of a block; groups of lanes; parts of a round
     __shared__ float4 red[AT_ONCE][WARPS][J][32];
@@ -280,11 +280,11 @@ __global__ void __launch_bounds__(MERGE_THREADS) prefix_merge_kernel(PrefixMerge
     const int most = live ? a.splits + (chunked ? a.own.splits : a.own_splits) : 0;
     // Where part i of the row lies, counted in rows of its array.
     auto own_at = [&](int i) { return chunked ? row * a.own.splits + i - a.splits : (int64_t)(i - a.splits) * a.rows + row; };
-    float lse[MERGE_EACH];
-    float4 x[MERGE_EACH][J];
+    float lse[EACH];
+    float4 x[EACH][J];
     auto ask = [&](int i0, int end) {
 #pragma unroll
-        for (int e = 0; e < MERGE_EACH; ++e) {
+        for (int e = 0; e < EACH; ++e) {
             const int i = i0 + e * STEP + slot;
             lse[e] = -INFINITY;
 #pragma unroll
@@ -326,16 +326,16 @@ __global__ void __launch_bounds__(MERGE_THREADS) prefix_merge_kernel(PrefixMerge
         for (int j = 0; j < J; ++j) { num[j].x *= by; num[j].y *= by; num[j].z *= by; num[j].w *= by; }
     };
     auto weight = [](float x, float top) { return expf(x - (top == -INFINITY ? 0.f : top)); };
-    for (int i0 = 0; i0 < parts; i0 += MERGE_EACH * STEP) {
+    for (int i0 = 0; i0 < parts; i0 += EACH * STEP) {
         if (i0 > 0) ask(i0, parts);
         float now = top;
 #pragma unroll
-        for (int e = 0; e < MERGE_EACH; ++e)
+        for (int e = 0; e < EACH; ++e)
             if (there(i0 + e * STEP + slot, lse[e])) now = fmaxf(now, lse[e]);
         scaled(weight(top, now));
         top = now;
 #pragma unroll
-        for (int e = 0; e < MERGE_EACH; ++e) {
+        for (int e = 0; e < EACH; ++e) {
             if (!there(i0 + e * STEP + slot, lse[e])) continue;
             const float w = weight(lse[e], top);
             den += w;
@@ -416,19 +416,21 @@ cudaError_t generic_t(const PrefixArgs &a, dim3 grid, cudaStream_t stream) {
     return a.d % V == 0 && vectors(a.k) && vectors(a.v) && vectors(View4{a.q, 0, a.q_sb, a.q_sh, a.q_sd}) ? generic_v<T, V>(a, grid, stream) : generic_v<T, 1>(a, grid, stream);
 }
 
-template <typename T, int WARPS>
+template <typename T, int WARPS, int EACH>
 cudaError_t merge_w(const PrefixMergeArgs &a, cudaStream_t stream) {
     constexpr int AT_ONCE = MERGE_THREADS / 32 / WARPS;
     const int64_t blocks = (a.rows + AT_ONCE - 1) / AT_ONCE;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-    const auto kernel = a.d <= 64 ? prefix_merge_kernel<T, WARPS, 16, 1> : a.d <= 128 ? prefix_merge_kernel<T, WARPS, 32, 1> : prefix_merge_kernel<T, WARPS, 32, 2>;
+    const auto kernel = a.d <= 64 ? prefix_merge_kernel<T, WARPS, EACH, 16, 1> : a.d <= 128 ? prefix_merge_kernel<T, WARPS, EACH, 32, 1> : prefix_merge_kernel<T, WARPS, EACH, 32, 2>;
     return launch_beside(kernel, dim3((unsigned)blocks), MERGE_THREADS, 0, stream, true, a);
 }
-// Four warps a row where one would not have all parts on their way at once, and rows are few.
+// Several warps a row where one would not have all parts on their way at once, and rows are few.  (The step, us, one warp of eight parts | two of
+// four | four of four: 2048 rows of 128, 42.3 | 42.4 | 43.3, 1536 34.1 | 33.7 | 34.8, 512 31.0 | 29.8 | 28.4, 128 35.6 | 32.7 | 29.4.)
 template <typename T>
 cudaError_t merge_t(const PrefixMergeArgs &a, cudaStream_t stream) {
     const int parts = a.splits + (a.own.s > 0 ? std::max(a.own_splits, a.own_splits > 0 ? 0 : a.own.splits) : 0);
-    return parts > MERGE_EACH * (a.d <= 64 ? 2 : 1) && a.rows <= 148 * 16 ? merge_w<T, 4>(a, stream) : merge_w<T, 1>(a, stream);
+    if (parts <= 8 * (a.d <= 64 ? 2 : 1) || a.rows > 148 * 16) return merge_w<T, 1, 8>(a, stream);
+    return a.rows <= 148 * 8 ? merge_w<T, 4, 4>(a, stream) : merge_w<T, 2, 4>(a, stream);
 }
 
 int64_t generic_units(int n, int each, int hq, int hkv) { return (int64_t)n * hkv * (((int64_t)each * (hq / hkv) + ROWS - 1) / ROWS); }

@@ -285,3 +285,15 @@ def test_far_offsets():
         values[:, :200] = x["pv"]
     got = attention_decode_shared(x["q"], big, values, x["k"], x["v"], None, index(plens))
     check(got, {**x, "pk": big[:, :200], "pv": values[:, :200]}, plens, [10] * 6)
+
+
+@pytest.mark.parametrize("dtype", list(TORCH))
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n,each,p,hq", [(2, 20, 1500, 32), (1, 2, 5000, 8), (1, 80, 300, 32)])
+def test_many_parts(n, each, p, hq, d, dtype):
+    """Long own caches and prompts, so that a row has parts for several rounds, by all numbers of rows."""
+    s = 3000 if n * each < 80 else 900
+    x = inputs(dtype, n, each, p, s, hq, 1, d, seed=170)
+    lens = np.random.default_rng(d).integers(0, s + 1, n * each)
+    lens[0], lens[1] = s, 0
+    check(attention_decode_shared(x["q"], x["pk"], x["pv"], x["k"], x["v"], index(lens)), x, [p] * n, list(map(int, lens)))
