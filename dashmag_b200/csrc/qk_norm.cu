@@ -637,10 +637,12 @@ __global__ void __launch_bounds__(THREADS) qk_norm_elements_kernel(NormArgs a, i
     }
 }
 
-// The weight's gradient from the blocks' rows, in their order: a block 32 columns of one tensor.
+// The weight's gradient from the blocks' rows, in their order: a block 32 columns of one tensor, as many warps as it may have, so that each has
+// one trip or two to memory (the gradient of 1000 tokens of 16 / 4 heads of 128, 8 warps | 32: 12.0 | 10.0 us).
+constexpr int SUM_WARPS = 32;
 template <typename TW>
-__global__ void __launch_bounds__(THREADS) qk_norm_sum_kernel(NormArgs a, int blocks_q, int blocks) {
-    __shared__ float red[WARPS][32];
+__global__ void __launch_bounds__(SUM_WARPS * 32) qk_norm_sum_kernel(NormArgs a, int blocks_q, int blocks) {
+    __shared__ float red[SUM_WARPS][32];
     wait_before();
     const bool is_k = blockIdx.y == 1;
     const NormTensor &t = is_k ? a.k : a.q;
@@ -649,12 +651,13 @@ __global__ void __launch_bounds__(THREADS) qk_norm_sum_kernel(NormArgs a, int bl
     float sum = 0.f;
     if (t.dw && c < a.d) {
 #pragma unroll 8
-        for (int i = b0 + warp; i < b1; i += WARPS) sum += a.part[(int64_t)i * a.d + c];
+        for (int i = b0 + warp; i < b1; i += SUM_WARPS) sum += a.part[(int64_t)i * a.d + c];
     }
     red[warp][lane] = sum;
     __syncthreads();
     if (warp != 0 || !t.dw || c >= a.d) return;
-    for (int i = 1; i < WARPS; ++i) sum += red[i][lane];
+#pragma unroll
+    for (int i = 1; i < SUM_WARPS; ++i) sum += red[i][lane];
     static_cast<TW *>(t.dw)[c] = Num<TW>::from_f32(sum);
 }
 
@@ -829,9 +832,9 @@ cudaError_t launch_qk_norm_backward(int dtype, const NormArgs &given, cudaStream
     if (e != cudaSuccess || (!a.q.dw && !a.k.dw)) return e;
     *launches += 1;
     const dim3 grid((unsigned)((a.d + 31) / 32), 2);
-    if (dtype == 0 || a.w_f32) return launch_beside(qk_norm_sum_kernel<float>, grid, THREADS, 0, stream, true, a, p.blocks_q, p.blocks);
-    if (dtype == 1) return launch_beside(qk_norm_sum_kernel<__nv_bfloat16>, grid, THREADS, 0, stream, true, a, p.blocks_q, p.blocks);
-    return launch_beside(qk_norm_sum_kernel<__half>, grid, THREADS, 0, stream, true, a, p.blocks_q, p.blocks);
+    if (dtype == 0 || a.w_f32) return launch_beside(qk_norm_sum_kernel<float>, grid, SUM_WARPS * 32, 0, stream, true, a, p.blocks_q, p.blocks);
+    if (dtype == 1) return launch_beside(qk_norm_sum_kernel<__nv_bfloat16>, grid, SUM_WARPS * 32, 0, stream, true, a, p.blocks_q, p.blocks);
+    return launch_beside(qk_norm_sum_kernel<__half>, grid, SUM_WARPS * 32, 0, stream, true, a, p.blocks_q, p.blocks);
 }
 
 cudaError_t read_qk_norm_status(unsigned int *status, bool clear) {
