@@ -306,7 +306,7 @@ __device__ __forceinline__ void leave_part(const NormArgs &a, const Place<V, LPH
 // The weight's gradient: a lane's sums are one tensor's columns and stay in registers to the end.
 __device__ unsigned int g_qk_norm_status = 0;   // sticky: non-zero once a bounded wait has run out
 
-// Of a stage: HG loads of 32 / LPH heads each.  Four warps a block and three blocks a multiprocessor: 168 registers, with which nothing spills.
+// Of a stage: HG loads of 32 / LPH heads each.  Four warps a block and three blocks a multiprocessor: 168 registers, with which next to nothing spills (backward in 16 bits one to five words).
 template <bool BACK> struct Ring {
     static constexpr int HG = BACK ? 4 : 8, STAGES = 2, WARPS = 4, BLOCKS = 3;
 };
@@ -705,7 +705,7 @@ Plan plan_of(int dtype, const NormArgs &a, bool back) {
         r.heads = std::min(t.heads, ng * hg);
         while (r.heads > ng && stage_bytes(back, r.heads, 1, a.d, a.dim, eb) > STAGE_MOST) r.heads -= ng;
         r.units = r.heads ? (t.heads + r.heads - 1) / r.heads : 0;
-        r.tokens = r.heads ? std::max(1, std::min(32, ng * hg / r.heads)) : 1;
+        r.tokens = r.units == 1 ? std::max(1, std::min(32, ng * hg / r.heads)) : 1;
         r.tokens = (int)std::min<int64_t>(r.tokens, std::max<int64_t>(1, tokens / (room * nw / 2)));   // (few tokens: rather more warps)
         while (r.tokens > 1 && stage_bytes(back, r.heads * r.tokens, r.tokens, a.d, a.dim, eb) > STAGE_MOST) --r.tokens;
         r.stage = stage_bytes(back, r.heads * r.tokens, r.tokens, a.d, a.dim, eb);
