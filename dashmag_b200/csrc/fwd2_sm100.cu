@@ -99,12 +99,18 @@ template <> struct Pack<__nv_bfloat16> {
         __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<uint32_t *>(&v);
     }
+    // What the rounding of two values lost, rounded.
+    static __device__ __forceinline__ uint32_t rest(float a, float b, uint32_t v) { return two(a - __uint_as_float(v << 16), b - __uint_as_float(v & 0xffff0000u)); }
 };
 template <> struct Pack<__half> {
     static constexpr int FMT = 0;
     static __device__ __forceinline__ uint32_t two(float a, float b) {
         __half2 v = __floats2half2_rn(a, b);
         return *reinterpret_cast<uint32_t *>(&v);
+    }
+    static __device__ __forceinline__ uint32_t rest(float a, float b, uint32_t v) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&v));
+        return two(a - x.x, b - x.y);
     }
 };
 
@@ -132,6 +138,8 @@ __device__ __noinline__ void rescale_accumulator(uint32_t taddr, float factor) {
 // PREFIX: split, over a decoding step's shared prompts (prefix.cu): batch element = prompt, token = sequence of it, intervals
 // from a.reach.  What lies past a prompt's end may be anything: its scores are masked as any others, and its values, which P's zeros would
 // not keep out if they are not finite, are cleared in shared memory before they are multiplied.
+// P is the sum of two 16-bit values there, the second what the rounding of the first lost, as in the decoding step itself (decode.cu): the
+// step over shared prompts rounds no more than the step over joined caches.
 enum FwdForm { WHOLE, SPLITS, PREFIXES };
 template <typename T, int HD, FwdForm FORM>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -352,6 +360,11 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 for (int ks = 0; ks < SN / 16; ++ks)
                     umma_f16_ts_words(col_o, col_s + half * SN + ks * 8, v_lo + tile_at(st, half) + ((ks * 2048) >> 4), v_hi, IDESC_O,
                                       (u > 0 || ks > 0) ? 1u : 0u);
+                if constexpr (PREFIX) {
+#pragma unroll
+                    for (int ks = 0; ks < SN / 16; ++ks)
+                        umma_f16_ts_words(col_o, col_s + half * SN + SN / 2 + ks * 8, v_lo + tile_at(st, half) + ((ks * 2048) >> 4), v_hi, IDESC_O, 1u);
+                }
                 if (more) {
                     qk(st ^ 1, half);
                     umma_commit(FWD2_BAR(s_full) + 8 * (2 * t + half));
@@ -488,19 +501,21 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             if (!solo && (t == 1 || u > 0)) {
                 if (!__all_sync(0xffffffffu, mbar_wait(BAR(sh.bar.turn[warp & 3][t]), (t == 1 ? u : u - 1) & 1))) { failed = true; break; }
             }
-            // P over the first 32 columns of the buffer this thread has read (two 16-bit values a column).
+            // P over the first 32 columns of the buffer this thread has read (two 16-bit values a column); PREFIX: its second part over the others.
             float2 sum2[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
             for (int cc = 0; cc < SN / 32; ++cc) {
-                uint32_t pk[16];
+                uint32_t pk[16], pl[PREFIX ? 16 : 1];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const float2 x = fma2(make_float2(s[cc * 32 + 2 * e], s[cc * 32 + 2 * e + 1]), sl2, neg2);
                     const float p0 = ex2(x.x), p1 = ex2(x.y);
                     sum2[e & 3] = add2(sum2[e & 3], make_float2(p0, p1));
                     pk[e] = Pack<T>::two(p0, p1);
+                    if constexpr (PREFIX) pl[e] = Pack<T>::rest(p0, p1, pk[e]);
                 }
                 tmem_st16(t_lane + COL_S(t, buf) + cc * 16, pk);
+                if constexpr (PREFIX) tmem_st16(t_lane + COL_S(t, buf) + SN / 2 + cc * 16, pl);
             }
             __syncwarp();
             if (!solo && lane == 0) mbar_arrive(BAR(sh.bar.turn[warp & 3][t ^ 1]));   // the other tile's turn

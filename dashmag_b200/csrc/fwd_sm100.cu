@@ -84,6 +84,8 @@ template <> struct Pack<__nv_bfloat16> {
         __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<uint32_t *>(&v);
     }
+    // What the rounding of two values lost, rounded.
+    static __device__ __forceinline__ uint32_t rest(float a, float b, uint32_t v) { return two(a - __uint_as_float(v << 16), b - __uint_as_float(v & 0xffff0000u)); }
 };
 template <> struct Pack<__half> {
     static constexpr int FMT = 0;
@@ -91,12 +93,16 @@ template <> struct Pack<__half> {
         __half2 v = __floats2half2_rn(a, b);
         return *reinterpret_cast<uint32_t *>(&v);
     }
+    static __device__ __forceinline__ uint32_t rest(float a, float b, uint32_t v) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&v));
+        return two(a - x.x, b - x.y);
+    }
 };
 
 }  // namespace
 
 // SPLIT: the block sweeps one of a.splits runs of its tile's keys and leaves a part for the merge (as in the two-tile kernel).
-// PREFIX: split, over a decoding step's shared prompts (as in the two-tile kernel, values past a prompt's end cleared too).
+// PREFIX: split, over a decoding step's shared prompts (as in the two-tile kernel, values past a prompt's end cleared and P in two parts too).
 enum FwdForm { WHOLE, SPLITS, PREFIXES };
 template <typename T, int HD, FwdForm FORM>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -254,6 +260,11 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                         // A = P in tensor memory, over the S buffer it came from: 16 keys = 8 columns a step.
                         umma_f16_ts(tmem + 256, tmem + st * BN + ks * 8, desc_at(v_desc, ks * 2048), IDESC_O,
                                     (i > 0 || ks > 0) ? 1u : 0u);
+                    if constexpr (PREFIX) {
+#pragma unroll
+                        for (int ks = 0; ks < BN / 16; ++ks)
+                            umma_f16_ts(tmem + 256, tmem + st * BN + BN / 2 + ks * 8, desc_at(v_desc, ks * 2048), IDESC_O, 1u);
+                    }
                     umma_commit(v_empty);
                     umma_commit(s_empty);   // the S buffer (now P) may be overwritten by S of tile i + 2
                     umma_commit(o_ready);
@@ -359,6 +370,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             const float neg = none ? -INFINITY : m_ref == -INFINITY ? 0.f : -__fmul_rn(m_ref, a.scale_log2);
 
             uint32_t pk[BN / 2];  // P of this row, two keys per 32-bit column
+            uint32_t pl[PREFIX ? BN / 2 : 1];   // PREFIX: what its rounding lost
             const float2 sl2 = make_float2(a.scale_log2, a.scale_log2), neg2 = make_float2(neg, neg);
             float2 sum2[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -373,7 +385,10 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                     sum2[e] = add2(sum2[e], make_float2(p[2 * e], p[2 * e + 1]));
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) pk[cc * 4 + e] = Pack<T>::two(p[2 * e], p[2 * e + 1]);
+                for (int e = 0; e < 4; ++e) {
+                    pk[cc * 4 + e] = Pack<T>::two(p[2 * e], p[2 * e + 1]);
+                    if constexpr (PREFIX) pl[cc * 4 + e] = Pack<T>::rest(p[2 * e], p[2 * e + 1], pk[cc * 4 + e]);
+                }
             }
             {
                 const float2 t = add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3]));
@@ -398,9 +413,13 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                     tc_fence_before_sync();
                 }
             }
-            // P goes back into the first 64 columns of the S buffer it was read from.
+            // P goes back into the first 64 columns of the S buffer it was read from (PREFIX: its second part into the others).
             tmem_st32(t_lane + st * BN, *reinterpret_cast<uint32_t(*)[32]>(&pk[0]));
             tmem_st32(t_lane + st * BN + 32, *reinterpret_cast<uint32_t(*)[32]>(&pk[32]));
+            if constexpr (PREFIX) {
+                tmem_st32(t_lane + st * BN + 64, *reinterpret_cast<uint32_t(*)[32]>(&pl[0]));
+                tmem_st32(t_lane + st * BN + 96, *reinterpret_cast<uint32_t(*)[32]>(&pl[32]));
+            }
             tmem_st_wait();
             tc_fence_before_sync();
             mbar_arrive(BAR(sh.bar.p_full, st));
