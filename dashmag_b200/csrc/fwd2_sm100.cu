@@ -538,6 +538,10 @@ fwd2_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 if (row < a.tq) a.part_lse[at] = -INFINITY;
             } else if (__all_sync(0xffffffffu, mbar_wait(BAR(sh.bar.o_done[t]), 0))) {
                 tc_fence_after_sync();
+                // (PREFIX: a row that sees none of the run's keys has left nothing, whatever its exponentials came to: those of a key past the
+                // prompt's end that is not finite are NaN against -inf too.  A row that sees some sees the last, so that the look for hidden
+                // keys is taken wherever the run's last sub-step has keys past the end.)
+                if (PREFIX && max(lo, kmin) >= min(hi, kmax)) l = 0.f;
                 const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll 1
                 for (int c = 0; c < HD / 32; ++c) {

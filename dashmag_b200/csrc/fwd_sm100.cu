@@ -442,6 +442,8 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             }
         } else if (__all_sync(0xffffffffu, mbar_wait(o_ready, (n_tiles - 1) & 1))) {
             tc_fence_after_sync();
+            // (PREFIX: a row that sees none of the run's keys has left nothing, as in the two-tile kernel.)
+            if (PREFIX && max(lo, kmin) >= min(hi, kmax)) l = 0.f;
             const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll 1
             for (int c = 0; c < HD / 32; ++c) {
