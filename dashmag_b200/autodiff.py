@@ -17,6 +17,7 @@ import torch
 from . import attention as A
 from .contract import AttentionMask, AttentionOptions
 from .qk_norm import QkNorm
+from .rope import Rope
 
 
 class AttentionNode(torch.autograd.Function):
@@ -107,21 +108,28 @@ def attention_decode(query, key, value, cache_lengths: Optional[torch.Tensor] = 
     return reference_decode(query, key, value, cache_lengths, options)
 
 
+def _versioned(tensor):
+    """``tensor`` as a node may save it: one made in inference mode has no version to be checked, so a copy."""
+    return tensor.clone() if tensor is not None and tensor.is_inference() else tensor
+
+
 class QkNormNode(torch.autograd.Function):
-    """The norm of a layer's query and key with the rotation: its state is the call's inputs, its backward the written-out pass."""
+    """The norm of a layer's query and key with the rotation: its state is the call's inputs, its backward the written-out pass.  The rotation's
+    tables and the positions or offsets are of that state too: the backward turns by them, so one written again before it is refused."""
 
     @staticmethod
     def forward(ctx, query, key, query_weight, key_weight, norm: QkNorm, where: dict):
-        ctx.save_for_backward(query, key, query_weight, key_weight)
-        ctx.norm, ctx.where = norm, where
+        ctx.index = next((name for name in ("positions", "cu_seqlens") if name in where), None)
+        ctx.save_for_backward(query, key, query_weight, key_weight, _versioned(norm.rope.cos), _versioned(norm.rope.sin), _versioned(where.get(ctx.index)))
+        ctx.eps, ctx.where = norm.eps, {name: x for name, x in where.items() if name != ctx.index}
         return norm.forward_of(query, key, where)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_query, grad_key):
-        query, key, query_weight, key_weight = ctx.saved_tensors
-        norm = QkNorm(ctx.norm.rope, query_weight, key_weight, ctx.norm.eps)
-        grads = norm.backward_of(query, key, grad_query, grad_key, ctx.where)
+        query, key, query_weight, key_weight, cos, sin, index = ctx.saved_tensors
+        norm = QkNorm(Rope.from_tables(cos, sin), query_weight, key_weight, ctx.eps)
+        grads = norm.backward_of(query, key, grad_query, grad_key, ctx.where if index is None else {**ctx.where, ctx.index: index})
         return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None)
 
 
