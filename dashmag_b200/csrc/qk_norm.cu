@@ -238,8 +238,8 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(NormArgs a, int units_
         for (int i = 0; i < V / 2; ++i) {
             k1[i] = ptx::mul2(pair<V>(w.w1, i), pair<V>(turn.c1, i));
             k2[i] = ptx::mul2(pair<V>(w.w2, i), pair<V>(turn.c2, i));
-            z1[i] = neg2(ptx::mul2(pair<V>(w.w2, i), pair<V>(turn.s1, i)));
-            z2[i] = ptx::mul2(pair<V>(w.w1, i), pair<V>(turn.s2, i));
+            z1[i] = at.rotated ? neg2(ptx::mul2(pair<V>(w.w2, i), pair<V>(turn.s1, i))) : both(0.f);
+            z2[i] = at.rotated ? ptx::mul2(pair<V>(w.w1, i), pair<V>(turn.s2, i)) : both(0.f);
         }
     }
     const float inv_d = 1.f / a.d;
@@ -262,6 +262,13 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(NormArgs a, int units_
             for (int i = 0; i < V / 2; ++i) {
                 put<V>(x1[g], i, ptx::mul2(ptx::fma2(u1[i], k1[i], ptx::mul2(u2[i], z1[i])), both(r)));
                 put<V>(x2[g], i, ptx::mul2(ptx::fma2(u2[i], k2[i], ptx::mul2(u1[i], z2[i])), both(r)));
+            }
+            if (r == 0.f && !at.rotated) {   // an infinity in the head: columns behind the rotated ones are no partners, and it times a sine of zero no zero
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i) {
+                    put<V>(x1[g], i, ptx::mul2(ptx::mul2(u1[i], k1[i]), both(r)));
+                    put<V>(x2[g], i, ptx::mul2(ptx::mul2(u2[i], k2[i]), both(r)));
+                }
             }
         }
         store<T, V>(out + g * NG * a.d, x1[g]);
@@ -353,8 +360,8 @@ struct Factors {
                 const float2 w1 = pair<V>(w.w1, i), w2 = pair<V>(w.w2, i);
                 k1[i] = ptx::mul2(k1[i], w1);
                 k2[i] = ptx::mul2(k2[i], w2);
-                z1[i] = ptx::mul2(z1[i], w2);
-                z2[i] = ptx::mul2(z2[i], w1);
+                z1[i] = at.rotated ? ptx::mul2(z1[i], w2) : both(0.f);
+                z2[i] = at.rotated ? ptx::mul2(z2[i], w1) : both(0.f);
             }
         }
     }
@@ -464,9 +471,13 @@ __global__ void __launch_bounds__(Ring<BACK>::WARPS * 32, Ring<BACK>::BLOCKS) qk
                             u2[i] = pair<V>(x2, i);
                             square = ptx::fma2(u1[i], u1[i], ptx::fma2(u2[i], u2[i], square));
                             if constexpr (BACK) {
-                                const float2 v1 = pair<V>(y1, i), v2 = pair<V>(y2, i);
-                                g1[i] = ptx::fma2(v1, f.k1[i], ptx::mul2(v2, f.z2[i]));
-                                g2[i] = ptx::fma2(v2, f.k2[i], ptx::mul2(v1, f.z1[i]));
+                                g1[i] = pair<V>(y1, i);
+                                g2[i] = pair<V>(y2, i);
+                                if (at.rotated) {   // (no partners behind the rotated ones: an infinite one times a sine of zero would be no zero)
+                                    const float2 v1 = g1[i], v2 = g2[i];
+                                    g1[i] = ptx::fma2(v1, f.k1[i], ptx::mul2(v2, f.z2[i]));
+                                    g2[i] = ptx::fma2(v2, f.k2[i], ptx::mul2(v1, f.z1[i]));
+                                }
                                 along = ptx::fma2(ptx::mul2(g1[i], pair<V>(w.w1, i)), u1[i], ptx::fma2(ptx::mul2(g2[i], pair<V>(w.w2, i)), u2[i], along));
                             }
                         }
@@ -486,6 +497,13 @@ __global__ void __launch_bounds__(Ring<BACK>::WARPS * 32, Ring<BACK>::BLOCKS) qk
                             } else {
                                 put<V>(y1, i, ptx::mul2(ptx::fma2(u1[i], f.k1[i], ptx::mul2(u2[i], f.z1[i])), both(r)));
                                 put<V>(y2, i, ptx::mul2(ptx::fma2(u2[i], f.k2[i], ptx::mul2(u1[i], f.z2[i])), both(r)));
+                            }
+                        }
+                        if (!BACK && r == 0.f && !at.rotated) {   // (an infinity in the head, as above)
+#pragma unroll
+                            for (int i = 0; i < V / 2; ++i) {
+                                put<V>(y1, i, ptx::mul2(ptx::mul2(u1[i], f.k1[i]), both(r)));
+                                put<V>(y2, i, ptx::mul2(ptx::mul2(u2[i], f.k2[i]), both(r)));
                             }
                         }
                     }
