@@ -391,7 +391,8 @@ __global__ void __launch_bounds__(Ring<BACK>::WARPS * 32, Ring<BACK>::BLOCKS) qk
     // Warps in whole sets of `units`; what is left over (fewer than `units`) stands by.  (More units than warps: one set, in rounds.)
     const int warps = (is_k ? gridDim.x - blocks_q : blocks_q) * NW, number = (is_k ? blockIdx.x - blocks_q : blockIdx.x) * NW + wib;
     const int sets = max(warps / units, 1), set = warps >= units ? number / units : 0;
-    const int64_t tokens = set < sets && *reinterpret_cast<volatile unsigned int *>(&g_qk_norm_status) == 0 ? a.b * a.t : 0;
+    bool failed = *reinterpret_cast<volatile unsigned int *>(&g_qk_norm_status) != 0;   // (an earlier launch's: nothing is done)
+    const int64_t tokens = set < sets && !failed ? a.b * a.t : 0;
     const int64_t first = (int64_t)set * each, step = (int64_t)sets * each;
     const Place<V, LPH> at(a, lane);
     const int slots = plan.slots, beside = NG / slots, slot = lane / LPH / beside, part = lane / LPH % beside;   // tokens at once, heads of each
@@ -401,7 +402,6 @@ __global__ void __launch_bounds__(Ring<BACK>::WARPS * 32, Ring<BACK>::BLOCKS) qk
 #pragma unroll
     for (int i = 0; i < V / 2; ++i) d1[i] = d2[i] = both(0.f);
     unsigned phase = 0, pending = 0;   // bit per stage: the parity waited for next; whether its copies have been asked for and not met
-    bool failed = false;
     for (int unit = number - set * units; unit < units && !failed; unit += warps >= units ? units : warps) {
         const int h0 = unit * plan.heads, heads = min(plan.heads, t.heads - h0);
         unsigned what = 0;   // two bits per stage, of this lane's token: 0 a row of the tables is there, 1 the position is outside them, 2 a token of no sequence
@@ -516,6 +516,11 @@ __global__ void __launch_bounds__(Ring<BACK>::WARPS * 32, Ring<BACK>::BLOCKS) qk
         __syncwarp();
     }
     if (failed) {
+        // The sums are not what they should be, and look like none that are.
+        if constexpr (BACK) {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) d1[i] = d2[i] = both(nan_f32());
+        }
         // A copy did not come: the call has failed and says so; what else is on its way is waited for (again not for ever).
         for (int s = 0; s < STAGES; ++s)
             if (pending >> s & 1u) ptx::mbar_wait(bars + 8 * s, phase >> s & 1u);
