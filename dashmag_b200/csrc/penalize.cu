@@ -14,7 +14,7 @@
 // The history is read once per piece, from L2, so pieces are long - counters of 16 bits where no history overflows them - as far as the
 // blocks still fill the GPU evenly (chunks_of).  The pass is a read and a write of the logits, bound by HBM.
 // (Pieces of 8192 tokens held in registers, counters of 32 bits, four trips one after another: 256 rows of 100003 tokens with up to 8192
-// ids 85 us, one trip 58, now 42; clusters of eight blocks that read a share of the history each and count for one another in
+// ids 85 us, one trip 58, now 43; clusters of eight blocks that read a share of the history each and count for one another in
 // distributed shared memory 107: half of a text's ids are a few tokens, whose words all eight then wait for.)
 #include <algorithm>
 #include <type_traits>

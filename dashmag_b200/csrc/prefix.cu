@@ -6,7 +6,8 @@
 // with o_i the normalised output over one run of keys and lse_i the logarithm of its sum of exponentials.  The parts over the
 // sequences' own keys are those of the decoding step's split pass (decode.cu).  The parts over a prompt's keys come from a pass in
 // which all of the prompt's sequences are the rows of one product, each x group of them against every key-value head, so that a
-// prompt's keys are read from HBM once and not once per sequence: on the tensor cores the training forward's kernels take it
+// prompt's keys are read once per tile of rows (of 256, of 128 where heads are longer than 128; of 32 here) and not once per sequence: on the
+// tensor cores the training forward's kernels take it
 // (fwd2_sm100.cu, fwd_sm100.cu, the prefix form; 16-bit, head dimensions of whole 16-byte vectors), else the kernel here.  Own keys that the
 // split pass could only read element by element are swept the same way, every sequence a prompt of one.
 // The passes touch nothing of one another: that over the own keys, which HBM bounds, is launched beside the prompts', which is cut into no
@@ -263,7 +264,7 @@ __global__ void __launch_bounds__(THREADS) prefix_append_kernel(DecodeArgs a) {
 // parts' log-sum-exps and features at once, the first of them before it is known how many chunks the sequence's own keys make, and keeps
 // maximum, sum and outputs as the softmax does; the lanes' groups and the warps meet in order, so the bits repeat.
 // Bound by launch and latency, the parts being in L2: one trip to memory for most calls (one for the lengths, one for the log-sum-exps, one for the
-// parts: 32 prompts of sixteen answers, 8192 rows of 64, 56 us the step, now 51).
+// parts: 32 prompts of sixteen answers, 8192 rows of 64, 56 us the step, with one 51).
 constexpr int MERGE_THREADS = 128;
 
 template <typename T, int WARPS, int EACH, int LANES, int J>
@@ -425,7 +426,8 @@ cudaError_t merge_w(const PrefixMergeArgs &a, cudaStream_t stream) {
     return launch_beside(kernel, dim3((unsigned)blocks), MERGE_THREADS, 0, stream, true, a);
 }
 // Several warps a row where one would not have all parts on their way at once, and rows are few.  (The step, us, one warp of eight parts | two of
-// four | four of four: 2048 rows of 128, 42.3 | 42.4 | 43.3, 1536 34.1 | 33.7 | 34.8, 512 31.0 | 29.8 | 28.4, 128 35.6 | 32.7 | 29.4.)
+// four | four of four: 2048 rows of 128, 42.3 | 42.4 | 43.3, 1536 34.1 | 33.7 | 34.8, 512 31.0 | 29.8 | 28.4, 128 35.6 | 32.7 | 29.4, the
+// sweep over the prompts 1 to 3 us shorter than it is now, with probabilities of one part.)
 template <typename T>
 cudaError_t merge_t(const PrefixMergeArgs &a, cudaStream_t stream) {
     const int parts = a.splits + (a.own.s > 0 ? std::max(a.own_splits, a.own_splits > 0 ? 0 : a.own.splits) : 0);

@@ -708,7 +708,7 @@ Plan plan_of(int dtype, const NormArgs &a, bool back) {
     };
     Plan p{};
     // A lane's columns are 16 bytes where the halves that are paired are whole vectors, else (40 rotated of 80 in 16 bits) 8; the rows and the heads
-    // are whole vectors in any case, for the copies.  (16384 tokens of 16 / 4 such heads, element by element | so: 184 | 45 us, backward 411 | 69.)
+    // are whole vectors in any case, for the copies.  (16384 tokens of 16 / 4 such heads, element by element | so: 184 | 48 us, backward 411 | 70.)
     auto whole = [&](int columns) { return a.dim % (2 * columns) == 0 && a.d % (2 * columns) == 0; };
     p.columns = eb == 2 && !whole(v) ? v / 2 : v;
     const bool vec = whole(p.columns) && aligned(a.cos) && aligned(a.sin) && vectors(a.q) && vectors(a.k);

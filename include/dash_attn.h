@@ -271,8 +271,9 @@ int dash_rope_norm_backward(const dash_rope_tables *rope, const dash_rope_norm_p
  * The decoding step of a batch whose sequences share prompts: N prompts [N, P, Hkv, D], B = N * (sequences of a prompt), sequence
  * b continuing prompt b / (B / N).  Its query sees the prompt's keys (of which the first lengths[n] are there) and, behind them,
  * its own: the cache of dash_attn_decode_params, as in dash_attn_decode.  What dash_attn_decode gives on caches that hold the prompt's
- * rows and then the sequence's own, with every prompt's rows held and read once for all of its sequences.  The window's left
- * side counts over both.  k_new and v_new not NULL: the step appends, as dash_attn_decode_append does, to the sequence's own
+ * rows and then the sequence's own, probabilities held as finely (16-bit tensors: as the sum of two 16-bit values) but sums taken in another
+ * order; a prompt's rows are held once and read once for each tile of (sequence, head) rows, 128 or 256 on the tensor cores and 32 on the CUDA
+ * cores, instead of once for each sequence.  The window's left side counts over both.  k_new and v_new not NULL: the step appends, as dash_attn_decode_append does, to the sequence's own
  * cache.  A sequence that sees no key gets zeros.
  * What lies past a prompt's length, or past a sequence's, may be anything, NaN included.  (Under a window, keys of one prompt that
  * some of its sequences see and others do not must be finite.)
@@ -387,7 +388,7 @@ int dash_attn_kernels_take(const dash_attn_params *p, const void *q, const void 
 
 /*
  * Every wait inside the tensor-core kernels, and the norm's for its bulk copies, is bounded; one that runs out raises a sticky word on
- * the device instead of hanging, and later blocks and launches of those kernels then do nothing.
+ * the device instead of hanging, and later blocks and launches of those kernels then do nothing (a norm's weights' gradients come out NaN).
  * This reads that word (0 = healthy) and, with `clear` non-zero, resets it.  It synchronises with
  * the device, so it is for tests and for error paths, not for the hot loop.  Returns a negative
  * DASH_ATTN_* code if the word cannot be read.  The reference has no counterpart: its kernels
